@@ -1,0 +1,460 @@
+"""What the performance of the operators on rows is measured on: tokens sorted by expert and back, the learned relative
+position bias, dropout.
+
+`listed()` names fixed cases, `draw()` makes others of the same kinds and ranges. A case is prepared from a seed and run
+either in its plain form, from elementary torch operations in 32 bits, or (`own`) through the package's entry points.
+"""
+import bisect
+import importlib
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+DEV = "cuda:0"
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+SIZES = {"f32": 4, "f16": 2, "bf16": 2}
+MOST_ROUTED = 32768 * 8 * 2048      # the most elements of the sorted rows
+MOST_SCORES = 4 * 16 * 2048 * 2048  # the most elements of a bias with its batch
+MOST_DROPPED = 1 << 27
+
+
+# --- the cases ---------------------------------------------------------------------------------------------------
+
+def listed():
+    return [
+        # Serving: one token each of eight sequences finds its experts and comes back. Latency counts.
+        {"name": "route_step", "kind": "route", "tokens": 8, "choices": 2, "experts": 16, "k": 1024, "type": "bf16",
+         "index": 64, "lost": 0.0},
+        # A large batch of prompts over many small experts, every token's row copied to eight of them.
+        {"name": "route_large", "kind": "route", "tokens": 32768, "choices": 8, "experts": 256, "k": 2048,
+         "type": "bf16", "index": 64, "lost": 0.0},
+        # A ragged batch on one worker of several: a fifth of the choices are experts that other workers hold.
+        {"name": "route_ragged", "kind": "route", "tokens": 5003, "choices": 3, "experts": 61, "k": 1001,
+         "type": "f16", "index": 32, "lost": 0.2},
+        # Training: the gradients of the weights, of the experts' answers and of the tokens' rows.
+        {"name": "route_back", "kind": "route_back", "tokens": 16384, "choices": 4, "experts": 64, "k": 2048,
+         "type": "bf16", "lost": 0.0},
+        # The same in single precision with odd rows, some choices held elsewhere.
+        {"name": "route_back_ragged", "kind": "route_back", "tokens": 1999, "choices": 6, "experts": 40, "k": 777,
+         "type": "f32", "lost": 0.1},
+        # Long prompts: the bias is added to the scores of a batch.
+        {"name": "bias_scores", "kind": "bias", "batch": 4, "heads": 16, "q": 2048, "k": 2048, "buckets": 32,
+         "max_distance": 128, "two_sided": True, "scores": True, "at": False, "type": "bf16"},
+        # The bias by itself, made once for all layers of a model, at an odd length.
+        {"name": "bias_table", "kind": "bias", "batch": 1, "heads": 12, "q": 1023, "k": 1023, "buckets": 32,
+         "max_distance": 128, "two_sided": True, "scores": False, "at": False, "type": "f32"},
+        # Serving: one token each of 64 sequences of different lengths.
+        {"name": "bias_step", "kind": "bias", "batch": 64, "heads": 16, "q": 1, "k": 4096, "buckets": 32,
+         "max_distance": 128, "two_sided": False, "scores": True, "at": True, "type": "bf16"},
+        # Training: the gradient of the scores of a batch becomes the gradient of 32 rows.
+        {"name": "bias_back", "kind": "bias_back", "batch": 8, "heads": 16, "q": 1024, "k": 1024, "buckets": 32,
+         "max_distance": 128, "two_sided": True, "type": "bf16"},
+        # The same for answers that look at a longer text, at odd sizes.
+        {"name": "bias_back_odd", "kind": "bias_back", "batch": 1, "heads": 7, "q": 333, "k": 1777, "buckets": 64,
+         "max_distance": 500, "two_sided": False, "type": "f32"},
+        # Embedding rows of a million keys, as they were pulled; their gradients take the same call.
+        {"name": "dropout_rows", "kind": "dropout", "n": 1_000_000, "k": 64, "p": 0.1, "keys": True, "type": "f32"},
+        # The rows of a batch of tokens, of an odd length.
+        {"name": "dropout_odd", "kind": "dropout", "n": 4099, "k": 1001, "p": 0.25, "keys": False, "type": "bf16"},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _row_length(rng, longest):
+    """Half of the rows have a length that is a multiple of 16, the others any."""
+    k = _log(rng, 1, longest)
+    return max(16, k // 16 * 16) if rng.random() < 0.5 else k
+
+
+def draw(rng):
+    kind = rng.choice(["route", "route_back", "bias", "bias_back", "dropout"])
+    kind_type = rng.choice(sorted(TYPES))
+    if kind in ("route", "route_back"):
+        choices = rng.randint(1, 8)
+        k = _row_length(rng, 4096)
+        tokens = _log(rng, 1, 32768)
+        most = MOST_ROUTED // (1 if kind == "route" else 4) // (SIZES[kind_type] // 2)
+        tokens = max(1, min(tokens, most // (choices * k)))
+        case = {"kind": kind, "tokens": tokens, "choices": choices, "experts": _log(rng, choices, 512), "k": k,
+                "type": kind_type, "lost": rng.choice([0.0, 0.0, round(rng.uniform(0.01, 0.9), 3)])}
+        if kind == "route":
+            case["index"] = rng.choice([32, 64])
+        return case
+    if kind in ("bias", "bias_back"):
+        heads, two_sided = rng.randint(1, 32), rng.random() < 0.5
+        q, k = _log(rng, 1, 2048), _log(rng, 1, 8192)
+        buckets = rng.choice([8, 16, 32, 64, 128])
+        most = MOST_SCORES // (1 if kind == "bias" else 2) // (SIZES[kind_type] // 2)
+        k = max(1, min(k, most // (heads * q)))
+        batch = max(1, min(_log(rng, 1, 64), most // (heads * q * k)))
+        case = {"kind": kind, "batch": batch, "heads": heads, "q": q, "k": k, "buckets": buckets,
+                "max_distance": _log(rng, buckets, 2000), "two_sided": two_sided, "type": kind_type}
+        if kind == "bias":
+            case["scores"], case["at"] = rng.random() < 0.6, rng.random() < 0.4
+            if not case["scores"] and not case["at"]:
+                case["batch"] = 1
+        return case
+    k = _row_length(rng, 8192)
+    n = max(1, min(_log(rng, 1, 1_000_000), MOST_DROPPED // k))
+    return {"kind": kind, "n": n, "k": k, "p": round(rng.uniform(0.0, 0.6), 3), "keys": rng.random() < 0.5,
+            "type": kind_type}
+
+
+# --- inputs ------------------------------------------------------------------------------------------------------
+
+def _normal(g, *shape, scale=1.0, type=torch.float32):
+    return torch.randn(*shape, generator=g, device=DEV).mul_(scale).to(type)
+
+
+def _choices(case, g):
+    """The experts of every token, the likeliest first: some experts are more in demand than others."""
+    T, K, E = case["tokens"], case["choices"], case["experts"]
+    favour = torch.randn(E, generator=g, device=DEV)
+    score = torch.randn(T, E, generator=g, device=DEV).add_(favour)
+    top = torch.topk(score, K, dim=1)
+    weights = torch.softmax(top.values, 1).contiguous()
+    lost = torch.rand(T, K, generator=g, device=DEV) < case["lost"]
+    return top.indices.masked_fill(lost, -1).contiguous(), weights
+
+
+def _places(experts, E):
+    """What sorting by expert gives, for the cases that begin behind it."""
+    flat = experts.reshape(-1)
+    key = torch.where(flat < 0, E, flat)
+    order = torch.sort(key, stable=True).indices
+    place = torch.empty_like(order)
+    place[order] = torch.arange(order.numel(), device=DEV)
+    return torch.where(flat < 0, -1, place).to(torch.int32).view_as(experts)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    s = globals()["_prepare_" + case["kind"]](case, g)
+    s["case"] = case
+    return s
+
+
+def _prepare_route(case, g):
+    T, K, E, k, type = case["tokens"], case["choices"], case["experts"], case["k"], TYPES[case["type"]]
+    experts, weights = _choices(case, g)
+    n = T * K
+    return {"experts": experts if case["index"] == 64 else experts.to(torch.int32), "weights": weights,
+            "x": _normal(g, T, k, type=type), "answers": _normal(g, n, k, type=type),
+            "order": torch.empty(n, dtype=torch.int32, device=DEV),
+            "place": torch.empty(T, K, dtype=torch.int32, device=DEV),
+            "offsets": torch.empty(E + 1, dtype=torch.int32, device=DEV),
+            # (rows behind the last expert's are left as they are)
+            "rows": torch.zeros(n, k, dtype=type, device=DEV), "out": torch.empty(T, k, dtype=type, device=DEV)}
+
+
+def _prepare_route_back(case, g):
+    T, K, k, type = case["tokens"], case["choices"], case["k"], TYPES[case["type"]]
+    experts, weights = _choices(case, g)
+    n = T * K
+    return {"place": _places(experts, case["experts"]), "weights": weights, "grad": _normal(g, T, k, type=type),
+            "answers": _normal(g, n, k, type=type), "grad_rows": _normal(g, n, k, type=type),
+            "grad_answers": torch.zeros(n, k, dtype=type, device=DEV),
+            "grad_weights": torch.empty(T, K, device=DEV), "grad_x": torch.empty(T, k, dtype=type, device=DEV)}
+
+
+def _prepare_bias(case, g):
+    B, H, Q, K, type = case["batch"], case["heads"], case["q"], case["k"], TYPES[case["type"]]
+    s = {"table": _normal(g, case["buckets"], H), "out": torch.empty(B, H, Q, K, dtype=type, device=DEV),
+         "scores": _normal(g, B, H, Q, K, scale=3.0, type=type) if case["scores"] else None, "at": None}
+    if case["at"]:  # the sequences of a batch are at different positions
+        s["at"] = torch.randint(0, max(1, K - Q + 1), (B,), generator=g, device=DEV)
+    return s
+
+
+def _prepare_bias_back(case, g):
+    B, H, Q, K, type = case["batch"], case["heads"], case["q"], case["k"], TYPES[case["type"]]
+    return {"grad": _normal(g, B, H, Q, K, scale=0.01, type=type),
+            "grad_table": torch.empty(case["buckets"], H, device=DEV)}
+
+
+def _prepare_dropout(case, g):
+    n, k, type = case["n"], case["k"], TYPES[case["type"]]
+    keys = None
+    if case["keys"]:
+        keys = torch.randint(-(1 << 63), (1 << 63) - 1, (n,), generator=g, device=DEV)
+    return {"x": _normal(g, n, k, type=type), "keys": keys, "seed": int(g.initial_seed()) * 0x9E3779B97F4A7C15 % (1 << 64),
+            "out": torch.empty(n, k, dtype=type, device=DEV)}
+
+
+# --- one pass ----------------------------------------------------------------------------------------------------
+
+def run(state):
+    if own:
+        ops = importlib.import_module("ps-lite_amd").ops
+        return globals()["_own_" + state["case"]["kind"]](state, ops)
+    return globals()["_plain_" + state["case"]["kind"]](state)
+
+
+def _own_route(s, ops):
+    ops.route_sort(s["experts"], s["case"]["experts"], s["order"], s["place"], s["offsets"])
+    ops.route_rows(s["x"], s["place"], s["rows"])
+    ops.route_sum(s["answers"], s["place"], s["out"], weights=s["weights"])
+    return [s["order"], s["place"], s["offsets"], s["rows"], s["out"]]
+
+
+def _own_route_back(s, ops):
+    ops.route_sum_grad(s["grad"], s["answers"], s["place"], s["weights"], s["grad_answers"], s["grad_weights"])
+    ops.route_sum(s["grad_rows"], s["place"], s["grad_x"])
+    return [s["grad_answers"], s["grad_weights"], s["grad_x"]]
+
+
+def _own_bias(s, ops):
+    c = s["case"]
+    ops.relbias(s["table"], s["out"], c["max_distance"], two_sided=c["two_sided"], scores=s["scores"], q_at=s["at"])
+    return s["out"]
+
+
+def _own_bias_back(s, ops):
+    c = s["case"]
+    ops.relbias_grad(s["grad"], s["grad_table"], c["max_distance"], two_sided=c["two_sided"])
+    return s["grad_table"]
+
+
+def _own_dropout(s, ops):
+    ops.dropout(s["x"], s["out"], s["case"]["p"], s["seed"], keys=s["keys"])
+    return s["out"]
+
+
+def _plain_route(s):
+    E = s["case"]["experts"]
+    T, K = s["experts"].shape
+    flat = s["experts"].reshape(-1).long()
+    n = flat.numel()
+    here = (flat >= 0) & (flat < E)
+    key, order = torch.sort(torch.where(here, flat, E), stable=True)
+    rank = torch.arange(n, device=DEV)
+    place = torch.empty_like(order)
+    place[order] = rank
+    place = torch.where(here, place, -1)
+    offsets = torch.searchsorted(key, torch.arange(E + 1, device=DEV))
+    kept = key < E
+    rows = torch.where(kept[:, None], s["x"][order // K], 0)
+    terms = s["answers"].float()[place.clamp(min=0)].view(T, K, -1) * s["weights"][:, :, None]
+    out = torch.where(here.view(T, K, 1), terms, 0.0).sum(1).to(s["x"].dtype)
+    return [torch.where(kept, order, -1).to(torch.int32), place.view(T, K).to(torch.int32), offsets.to(torch.int32),
+            rows, out]
+
+
+def _plain_route_back(s):
+    T, K = s["place"].shape
+    place, type = s["place"].reshape(-1).long(), s["grad"].dtype
+    n, here = place.numel(), (place >= 0).view(T, K, 1)
+    at = place.clamp(min=0)
+    grad = s["grad"].float()[:, None, :]
+    grad_weights = torch.where(here, s["answers"].float()[at].view(T, K, -1) * grad, 0.0).sum(2)
+    grad_answers = torch.zeros(n + 1, grad.shape[2], dtype=type, device=DEV)  # (the last row takes what is not here)
+    grad_answers[torch.where(place >= 0, place, n)] = (s["weights"][:, :, None] * grad).view(n, -1).to(type)
+    grad_x = torch.where(here, s["grad_rows"].float()[at].view(T, K, -1), 0.0).sum(1).to(type)
+    return [grad_answers[:n], grad_weights, grad_x]
+
+
+def _borders(exact, steps, max_distance):
+    """The least distance of each of the buckets whose widths grow, in whole numbers."""
+    found = []
+    for c in range(1, steps):
+        bound = exact ** (steps - c) * max_distance ** c
+        found.append(bisect.bisect_left(range(max_distance + 1), bound, key=lambda d: d ** steps))
+    return found
+
+
+def _plain_buckets(rel, buckets, max_distance, two_sided):
+    side = buckets // 2 if two_sided else buckets
+    distance = rel.abs() if two_sided else (-rel).clamp(min=0)
+    exact = side // 2
+    borders = torch.tensor(_borders(exact, side - exact, max_distance), device=DEV, dtype=torch.int64)
+    bucket = torch.where(distance < exact, distance, exact + torch.bucketize(distance, borders, right=True))
+    return torch.where(rel > 0, side + bucket, bucket) if two_sided else bucket
+
+
+def _plain_bias(s):
+    c = s["case"]
+    at = torch.zeros(1, dtype=torch.int64, device=DEV) if s["at"] is None else s["at"]
+    rel = torch.arange(c["k"], device=DEV) - torch.arange(c["q"], device=DEV)[:, None] - at[:, None, None]
+    bias = s["table"].t()[:, _plain_buckets(rel, c["buckets"], c["max_distance"], c["two_sided"])].transpose(0, 1)
+    if s["scores"] is not None:
+        bias = s["scores"].float() + bias
+    return bias.to(s["out"].dtype)
+
+
+def _plain_bias_back(s):
+    c = s["case"]
+    rel = torch.arange(c["k"], device=DEV) - torch.arange(c["q"], device=DEV)[:, None]
+    bucket = _plain_buckets(rel, c["buckets"], c["max_distance"], c["two_sided"]).view(-1)
+    hot = (bucket[:, None] == torch.arange(c["buckets"], device=DEV)).float()
+    grad = s["grad"].float().sum(0).view(c["heads"], -1)
+    return (grad @ hot).t().contiguous()
+
+
+_LOW = 0xFFFFFFFF
+
+
+def _plain_dropout(s):
+    x, n, k, p = s["x"], s["case"]["n"], s["case"]["k"], s["case"]["p"]
+    key = torch.arange(n, device=DEV) if s["keys"] is None else s["keys"]
+    blocks = (k + 7) // 8
+    c0 = (key & _LOW)[:, None].expand(n, blocks)
+    c1 = ((key >> 32) & _LOW)[:, None].expand(n, blocks)
+    c2 = torch.arange(blocks, device=DEV).expand(n, blocks)
+    c3 = torch.zeros_like(c0)
+    k0, k1 = s["seed"] & _LOW, s["seed"] >> 32
+    for _ in range(10):  # Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers, as easy as 1, 2, 3)
+        a, b = c0 * 0xD2511F53, c2 * 0xCD9E8D57
+        c0, c1, c2, c3 = ((b >> 32) & _LOW) ^ c1 ^ k0, b & _LOW, ((a >> 32) & _LOW) ^ c3 ^ k1, a & _LOW
+        k0, k1 = (k0 + 0x9E3779B9) & _LOW, (k1 + 0xBB67AE85) & _LOW
+    words = torch.stack([c0, c1, c2, c3], 2)
+    halves = torch.stack([words & 0xFFFF, words >> 16], 3).view(n, 8 * blocks)[:, :k]
+    least = int(math.floor(p * 65536 + 0.5))
+    scale = torch.tensor(65536.0 / (65536 - least) if least < 65536 else 0.0, device=DEV)
+    return torch.where(halves >= least, x.float() * scale, 0.0).to(x.dtype)
+
+
+# --- what a pass gives, in 64 bits -------------------------------------------------------------------------------
+
+def exact(case, seed):
+    return globals()["_exact_" + case["kind"]](prepare(case, seed))
+
+
+def _exact_route(s):
+    E, (T, K) = s["case"]["experts"], s["experts"].shape
+    flat = s["experts"].reshape(-1).long()
+    n = flat.numel()
+    held = torch.nonzero((flat >= 0) & (flat < E)).view(-1)
+    counts = torch.bincount(flat[held], minlength=E)
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    mine = held[torch.argsort(flat[held] * n + held)]
+    order = torch.full((n,), -1, dtype=torch.int64, device=DEV)
+    order[:mine.numel()] = mine
+    place = torch.full((n,), -1, dtype=torch.int64, device=DEV)
+    place[mine] = torch.arange(mine.numel(), device=DEV)
+    rows = torch.zeros_like(s["rows"], dtype=torch.float64)
+    rows[:mine.numel()] = s["x"].double()[torch.div(mine, K, rounding_mode="floor")]
+    out = torch.zeros(T, s["case"]["k"], dtype=torch.float64, device=DEV)
+    for j in range(K):
+        at = place.view(T, K)[:, j]
+        some = torch.nonzero(at >= 0).view(-1)
+        out[some] += s["answers"][at[some]].double() * s["weights"][some, j, None].double()
+    return [order.to(torch.int32), place.view(T, K).to(torch.int32), offsets.to(torch.int32), rows, out]
+
+
+def _exact_route_back(s):
+    T, K = s["place"].shape
+    k = s["case"]["k"]
+    grad_answers = torch.zeros(T * K, k, dtype=torch.float64, device=DEV)
+    grad_weights = torch.zeros(T, K, dtype=torch.float64, device=DEV)
+    grad_x = torch.zeros(T, k, dtype=torch.float64, device=DEV)
+    grad = s["grad"].double()
+    for j in range(K):
+        at = s["place"][:, j].long()
+        some = torch.nonzero(at >= 0).view(-1)
+        at, mine = at[some], grad[some]
+        grad_answers[at] = s["weights"][some, j, None].double() * mine
+        grad_weights[some, j] = (s["answers"][at].double() * mine).sum(1)
+        grad_x[some] += s["grad_rows"][at].double()
+    return [grad_answers, grad_weights, grad_x]
+
+
+def _exact_bucket_table(case):
+    """The bucket of every distance up to the last border, one by one."""
+    side = case["buckets"] // 2 if case["two_sided"] else case["buckets"]
+    near, far, found = side // 2, case["max_distance"], []
+    steps = side - near
+    for d in range(far + 1):
+        b = d
+        if d >= near:
+            b = found[-1] if found and found[-1] >= near else near
+            while b < side - 1 and d ** steps >= near ** (side - b - 1) * far ** (b + 1 - near):
+                b += 1
+        found.append(b)
+    return side, torch.tensor(found, device=DEV)
+
+
+def _exact_buckets(case, rel):
+    side, table = _exact_bucket_table(case)
+    ahead = rel > 0
+    if case["two_sided"]:
+        return table[rel.abs().clamp(max=case["max_distance"])] + side * ahead
+    return table[torch.where(ahead, 0, -rel).clamp(max=case["max_distance"])]
+
+
+def _exact_bias(s):
+    c = s["case"]
+    out = torch.zeros(s["out"].shape, dtype=torch.float64, device=DEV)
+    if s["scores"] is not None:
+        out += s["scores"]
+    j = torch.arange(c["k"], device=DEV)[None, :]
+    i = torch.arange(c["q"], device=DEV)[:, None]
+    for b in range(c["batch"]):
+        bucket = _exact_buckets(c, j - i - (0 if s["at"] is None else s["at"][b]))
+        for h in range(c["heads"]):
+            out[b, h] += s["table"][:, h].double()[bucket]
+    return out
+
+
+def _exact_bias_back(s):
+    c = s["case"]
+    j = torch.arange(c["k"], device=DEV)[None, :]
+    bucket = _exact_buckets(c, j - torch.arange(c["q"], device=DEV)[:, None])
+    grad = s["grad"].sum(0, dtype=torch.float64)
+    return torch.stack([torch.where(bucket == u, grad, 0.0).sum((1, 2)) for u in range(c["buckets"])])
+
+
+def _exact_dropout(s):
+    n, k, p = s["case"]["n"], s["case"]["k"], s["case"]["p"]
+    blocks = -(-k // 8)
+    key = np.arange(n, dtype=np.uint64) if s["keys"] is None else s["keys"].cpu().numpy().view(np.uint64)
+    low, mul = np.uint64(_LOW), (np.uint64(0xD2511F53), np.uint64(0xCD9E8D57))
+    half = np.uint64(32)
+    drawn = np.empty((n, blocks, 8), np.uint16)
+    piece = max(1, (1 << 20) // blocks)
+    for first in range(0, n, piece):
+        rows = key[first:first + piece, None]
+        block = np.arange(blocks, dtype=np.uint64)[None, :]
+        c = [rows & low | 0 * block, rows >> half | 0 * block, block | 0 * rows, 0 * (rows | block)]
+        for r in range(10):
+            k0 = np.uint64(((s["seed"] & _LOW) + r * 0x9E3779B9) & _LOW)
+            k1 = np.uint64(((s["seed"] >> 32) + r * 0xBB67AE85) & _LOW)
+            a, b = c[0] * mul[0], c[2] * mul[1]
+            c = [(b >> half) ^ c[1] ^ k0, b & low, (a >> half) ^ c[3] ^ k1, a & low]
+        drawn[first:first + piece] = np.stack(c, 2).astype("<u4").view("<u2")
+    keep = torch.from_numpy(drawn.reshape(n, 8 * blocks)[:, :k].astype(np.int32)).to(DEV)
+    least = int(math.floor(p * 65536 + 0.5))
+    scale = 65536.0 / (65536 - least) if least < 65536 else 0.0
+    return torch.where(keep >= least, s["x"].double() * scale, 0.0)
+
+
+# --- what a pass cannot do without -------------------------------------------------------------------------------
+
+def work(case):
+    size = SIZES[case["type"]]
+    kind = case["kind"]
+    if kind in ("route", "route_back"):
+        T, K, k = case["tokens"], case["choices"], case["k"]
+        n, held = T * K, T * K * (1 - case["lost"])
+        if kind == "route":
+            # experts; order, place, offsets; the rows to the experts; their answers and the weights back
+            b = n * case["index"] // 8 + 8 * n + 4 * (case["experts"] + 1) + (T + held) * k * size
+            b += (held + T) * k * size + 4 * n
+            return {"bytes": int(b), "flops": int(2 * held * k)}
+        # the gradient, the answers and theirs, places, weights and theirs; the gradient of the rows back to the tokens
+        b = (T + 2 * held) * k * size + 12 * n + (held + T) * k * size
+        return {"bytes": int(b), "flops": int(4 * held * k)}
+    if kind in ("bias", "bias_back"):
+        cells = case["batch"] * case["heads"] * case["q"] * case["k"]
+        b = 4 * case["buckets"] * case["heads"] + cells * size
+        if kind == "bias" and case["scores"]:
+            b += cells * size
+        return {"bytes": b, "flops": cells}
+    cells = case["n"] * case["k"]
+    return {"bytes": 2 * cells * size + (8 * case["n"] if case["keys"] else 0), "flops": cells}
