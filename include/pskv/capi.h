@@ -297,6 +297,81 @@ int pskv_match(int device, const uint64_t* src_keys, size_t n_src, const float* 
                const uint64_t* dst_keys, size_t n_dst, float* dst_vals, size_t k, int op,
                uint64_t* matched, float* kernel_ms, int memkind);
 
+/* Operators on rows: what a worker does with rows between its pull and its push. They have no counterpart in the
+ * reference. Common to all of them:
+ *  - Buffers are device memory on `device`. Nothing is allocated and nothing waited for: the kernels are enqueued on `stream`
+ *    (a hipStream_t, NULL = the null stream) and may be captured into a graph (make the first call on a device outside any
+ *    capture). Calls share no state: several may run at once, from several threads, and two recorded graphs need only
+ *    working memory (`work`) of their own. Buffers stay the caller's to keep until the stream has run the call.
+ *  - What the host can see is checked before anything is enqueued (PSKV_EINVAL); indexes that lie in device memory are checked
+ *    by the kernels, so no value of theirs leads outside the buffers that the call was given.
+ *  - `type` is the type of the rows' elements. Sums are taken in float in a fixed order and rounded once (to nearest, ties to
+ *    even): the same inputs give the same bits. Strides count elements; the elements of a row lie side by side; rows may begin
+ *    anywhere that an element may. */
+#define PSKV_F32 0
+#define PSKV_F16 1
+#define PSKV_BF16 2
+
+/* Choices sorted by expert, stably: n choices (tokens x choices of each, row by row) of experts 0 .. E-1, numbers of `index_bits`
+ * (32 or 64) bits. Any other number is a choice that is not here (an expert of another worker).
+ *   offsets[E+1]  expert e's rows are [offsets[e], offsets[e+1])
+ *   place[n]      where choice i went, -1 when it is not here
+ *   order[n]      the choice that went to p (its token is order[p] / choices), -1 from offsets[E] on
+ * `work`: pskv_route_room(n, E) bytes, aligned to 4; none (NULL) where that is 0. */
+#define PSKV_ROUTE_MAX_EXPERTS 4096
+size_t pskv_route_room(size_t n, size_t E);
+int pskv_route_sort(int device, void* stream, const void* experts, int index_bits, size_t n, size_t E, int32_t* order,
+                    int32_t* place, int32_t* offsets, void* work, size_t work_bytes);
+
+/* Every token's row goes to its places: rows[place[t*choices + j]] = x[t]. Places outside [0, n_rows) are skipped, rows that no
+ * place names are left as they are. The gradient of x is pskv_route_sum of the rows' gradient, without weights. */
+int pskv_route_rows(int device, void* stream, int type, const void* x, size_t x_stride, size_t tokens, size_t k,
+                    const int32_t* place, size_t choices, void* rows, size_t rows_stride, size_t n_rows);
+
+/* The experts' answers come back: out[t] = sum over j of weights[t*choices + j] * rows[place[t*choices + j]], in the order
+ * of j. Places outside [0, n_rows) add nothing, whatever their weight; a token with no place gets zeros. weights == NULL: all are 1. */
+int pskv_route_sum(int device, void* stream, int type, const void* rows, size_t rows_stride, size_t n_rows,
+                   const int32_t* place, const float* weights, size_t choices, void* out, size_t out_stride, size_t tokens,
+                   size_t k);
+
+/* The gradient of pskv_route_sum: grad_rows[place] = weight * grad[t] (rows that no place names are left as they are) and
+ * grad_weights[t*choices + j] = <grad[t], rows[place]>, 0 for a place outside [0, n_rows). */
+int pskv_route_sum_grad(int device, void* stream, int type, const void* grad, size_t grad_stride, size_t tokens, size_t k,
+                        const void* rows, size_t rows_stride, size_t n_rows, const int32_t* place, const float* weights,
+                        size_t choices, void* grad_rows, size_t grad_rows_stride, float* grad_weights);
+
+/* The learned relative position bias: out[b,h,i,j] = scores[b,h,i,j] + table[bucket * H + h], where bucket is that of
+ * rel = (k_first + j) - (q_first + q_at[b] + i). `table` has `buckets` rows of H floats: what a pull of a PSKV_MODE_FIXED
+ * table with a key per bucket answers. Two-sided: half of the buckets (rounded down) are for rel <= 0, the others for rel > 0;
+ * one-sided: key positions behind the query's share bucket 0. Of the m buckets of a side the first m / 2 are for one distance
+ * each; the others widen in a geometric progression up to max_distance and the last one takes what lies beyond. Borders are
+ * found in whole numbers: bucket m / 2 + c begins at the least d with d^(m - m/2) >= (m/2)^(m - m/2 - c) max_distance^c.
+ * q_at (device, B entries) may be NULL: 0. scores may be NULL: the bias alone; scores may be out itself. Strides are host
+ * arrays of three (batch, head, row; the scores' may be 0, for what a batch or all heads share). Sums in float, one rounding. */
+#define PSKV_RELBIAS_MAX_BUCKETS 256
+int pskv_relbias(int device, void* stream, int type, const float* table, size_t buckets, size_t H, uint64_t max_distance,
+                 int two_sided, int64_t q_first, int64_t k_first, const int64_t* q_at, const void* scores,
+                 const int64_t* scores_stride, void* out, const int64_t* out_stride, size_t B, size_t Q, size_t K);
+/* The bucket of one relative position (host), or a negative PSKV_E* code. */
+int pskv_relbias_bucket(int64_t rel, size_t buckets, uint64_t max_distance, int two_sided);
+/* Its gradient: grad_table[u * H + h] = the sum of grad[b,h,i,j] over what bucket u was added to; 0 for a bucket that is not
+ * used: the values of a push to the table of the biases. `work`: pskv_relbias_grad_room(...) bytes, aligned to 4 (own_positions:
+ * whether q_at is given). */
+size_t pskv_relbias_grad_room(size_t buckets, size_t H, size_t B, size_t Q, size_t K, int own_positions);
+int pskv_relbias_grad(int device, void* stream, int type, const void* grad, const int64_t* grad_stride, size_t buckets, size_t H,
+                      uint64_t max_distance, int two_sided, int64_t q_first, int64_t k_first, const int64_t* q_at, size_t B,
+                      size_t Q, size_t K, float* grad_table, void* work, size_t work_bytes);
+
+/* Dropout of n rows of k elements: out = x * scale where the element is kept, 0 where it is dropped (whatever x is there). Nothing
+ * is stored: whether column c of a row is kept is drawn from the row's 64-bit key (keys[r], or first + r with keys == NULL),
+ * c and the seed, so the gradient is the same call on the gradient's rows, in any order, in any pieces. 16 bits b of
+ * Philox4x32-10 (key: seed low, high; counter: row key low, high, c / 8, 0; the 8 columns take the halves of its four words,
+ * low ones first) are compared with least = p * 65536 rounded to the nearest: kept where b >= least, scale = 65536 / (65536 -
+ * least). step (device, one word, may be NULL) is added to the seed: a recorded graph draws anew where the program changes it.
+ * out may be x itself. */
+int pskv_dropout(int device, void* stream, int type, const void* x, size_t x_stride, void* out, size_t out_stride, size_t n,
+                 size_t k, double p, uint64_t seed, const uint64_t* step, const uint64_t* keys, uint64_t first);
+
 /* Device-time accounting for roofline figures (no counterpart in the reference).
  * While enabled, every launch of the kernels listed above is bracketed by HIP
  * events on the table's stream. pskv_prof_read waits for the stream and returns

@@ -46,7 +46,9 @@ ERROR_NAMES = {
 SYMBOLS = [
     "pskv_table_create", "pskv_table_destroy", "pskv_push", "pskv_pull", "pskv_pushpull",
     "pskv_sync", "pskv_table_stream", "pskv_push_multi", "pskv_pull_multi", "pskv_pushpull_multi", "pskv_sync_multi", "pskv_replay_record", "pskv_replay_run", "pskv_replay_destroy", "pskv_size", "pskv_size_multi", "pskv_dump", "pskv_slice", "pskv_slice_noalloc", "pskv_server_ranges",
-    "pskv_assemble_pull", "pskv_match", "pskv_prof_enable", "pskv_prof_reset", "pskv_prof_read", "pskv_prof_samples",
+    "pskv_assemble_pull", "pskv_match", "pskv_route_room", "pskv_route_sort", "pskv_route_rows", "pskv_route_sum",
+    "pskv_route_sum_grad", "pskv_relbias", "pskv_relbias_bucket", "pskv_relbias_grad_room", "pskv_relbias_grad", "pskv_dropout",
+    "pskv_prof_enable", "pskv_prof_reset", "pskv_prof_read", "pskv_prof_samples",
     "pskv_copy_probe", "pskv_host_alloc", "pskv_host_free", "pskv_host_trim", "pskv_device_trim", "pskv_table_counters", "pskv_last_error",
     "pskv_version",
 ]
@@ -84,7 +86,8 @@ def _load_native():
         if raw is None:
             def raw(device):
                 return torch.cuda.current_stream(device).cuda_stream
-        native.setup(torch.Tensor, torch.int64, getattr(torch, "uint64", torch.int64), torch.float32, torch.int32, raw)
+        native.setup(torch.Tensor, torch.int64, getattr(torch, "uint64", torch.int64), torch.float32, torch.int32, raw,
+                     torch.float16, torch.bfloat16)
     _native = native
 
 
@@ -127,6 +130,19 @@ def load():
     lib.pskv_assemble_pull.argtypes = [i32, vp, sz, sz, vp, vp, vp, vp, vp, vp, sz, vp,
                                        ctypes.POINTER(sz), i32]
     lib.pskv_match.argtypes = [i32, vp, sz, vp, vp, sz, vp, sz, i32, ctypes.POINTER(u64), vp, i32]
+    i64, f64 = ctypes.c_int64, ctypes.c_double
+    lib.pskv_route_room.argtypes = [sz, sz]
+    lib.pskv_route_room.restype = sz
+    lib.pskv_route_sort.argtypes = [i32, vp, vp, i32, sz, sz, vp, vp, vp, vp, sz]
+    lib.pskv_route_rows.argtypes = [i32, vp, i32, vp, sz, sz, sz, vp, sz, vp, sz, sz]
+    lib.pskv_route_sum.argtypes = [i32, vp, i32, vp, sz, sz, vp, vp, sz, vp, sz, sz, sz]
+    lib.pskv_route_sum_grad.argtypes = [i32, vp, i32, vp, sz, sz, sz, vp, sz, sz, vp, vp, sz, vp, sz, vp]
+    lib.pskv_relbias.argtypes = [i32, vp, i32, vp, sz, sz, u64, i32, i64, i64, vp, vp, vp, vp, vp, sz, sz, sz]
+    lib.pskv_relbias_bucket.argtypes = [i64, sz, u64, i32]
+    lib.pskv_relbias_grad_room.argtypes = [sz, sz, sz, sz, sz, i32]
+    lib.pskv_relbias_grad_room.restype = sz
+    lib.pskv_relbias_grad.argtypes = [i32, vp, i32, vp, vp, sz, sz, u64, i32, i64, i64, vp, sz, sz, sz, vp, vp, sz]
+    lib.pskv_dropout.argtypes = [i32, vp, i32, vp, sz, vp, sz, sz, sz, f64, u64, vp, vp, u64]
     lib.pskv_prof_enable.argtypes = [vp, i32]
     lib.pskv_prof_reset.argtypes = [vp]
     lib.pskv_prof_read.argtypes = [vp, i32, ctypes.POINTER(u64), ctypes.POINTER(ctypes.c_double)]

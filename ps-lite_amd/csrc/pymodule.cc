@@ -12,6 +12,8 @@
 #include <numpy/arrayobject.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "pskv/capi.h"
 
 namespace {
@@ -20,7 +22,8 @@ namespace {
 PyObject* g_tensor_type = nullptr;
 PyObject *g_int64 = nullptr, *g_uint64 = nullptr, *g_float32 = nullptr, *g_int32 = nullptr;
 PyObject* g_raw_stream = nullptr;  // callable: device index -> hipStream_t of torch's current stream, as an int
-PyObject *s_dtype, *s_is_cuda, *s_is_contiguous, *s_numel, *s_data_ptr;
+PyObject *g_float16 = nullptr, *g_bfloat16 = nullptr;
+PyObject *s_dtype, *s_is_cuda, *s_is_contiguous, *s_numel, *s_data_ptr, *s_shape, *s_stride, *s_get_device;
 
 enum Kind { kNone = -1, kHost = PSKV_MEM_HOST, kDevice = PSKV_MEM_DEVICE };
 
@@ -368,11 +371,349 @@ PyObject* replay_run(PyObject*, PyObject* at) {
   return PyLong_FromLong(rc);
 }
 
-// setup(tensor_type, int64, uint64, float32, int32, raw_stream)
+// --- operators on rows --------------------------------------------------------------------------------------------------------
+// These check their tensors here, once, and refuse what the calls do not take with TypeError or ValueError.
+
+constexpr int kNoType = -1, kInt32 = 100, kInt64 = 101;  // beside PSKV_F32, PSKV_F16, PSKV_BF16
+
+// A tensor on a GPU, as the calls see it.
+struct Tensor {
+  const char* name;
+  void* ptr = nullptr;
+  int type = kNoType, dims = 0, device = -1;
+  int64_t n[4] = {1, 1, 1, 1}, by[4] = {0, 0, 0, 0};
+  explicit Tensor(const char* what) : name(what) {}
+  bool given() const { return type != kNoType; }
+  int64_t count() const { return n[0] * n[1] * n[2] * n[3]; }
+  // (torch leaves the strides of dimensions of one element to chance)
+  size_t stride(int d, int64_t if_one) const { return (size_t)(n[d] > 1 ? by[d] : if_one); }
+
+  bool fail(PyObject* error, const char* what) const {
+    PyErr_Format(error, "%s: %s", name, what);
+    return false;
+  }
+  bool take(PyObject* o, bool may_be_none = false) {
+    if (may_be_none && o == Py_None) return true;
+    if (!g_tensor_type || !PyObject_TypeCheck(o, reinterpret_cast<PyTypeObject*>(g_tensor_type)))
+      return fail(PyExc_TypeError, "a torch tensor is expected");
+    PyObject* at = PyObject_CallMethodNoArgs(o, s_get_device);
+    if (!at) return false;
+    device = (int)PyLong_AsLong(at);
+    Py_DECREF(at);
+    if (PyErr_Occurred()) return false;
+    PyObject* cuda = PyObject_GetAttr(o, s_is_cuda);
+    if (!cuda) return false;
+    Py_DECREF(cuda);
+    if (cuda != Py_True) return fail(PyExc_ValueError, "the tensor is not on the GPU");
+    PyObject* d = PyObject_GetAttr(o, s_dtype);
+    if (!d) return false;
+    Py_DECREF(d);
+    type = d == g_float32 ? PSKV_F32 : d == g_float16 ? PSKV_F16 : d == g_bfloat16 ? PSKV_BF16 : d == g_int32 ? kInt32
+           : d == g_int64 || d == g_uint64 ? kInt64 : kNoType;
+    if (type == kNoType) return fail(PyExc_TypeError, "not a type that a call takes");
+    PyObject* shape = PyObject_GetAttr(o, s_shape);
+    if (!shape) return false;
+    PyObject* steps = PyObject_CallMethodNoArgs(o, s_stride);
+    bool ok = steps && PyTuple_Check(shape) && PyTuple_Check(steps) && PyTuple_GET_SIZE(shape) == PyTuple_GET_SIZE(steps);
+    if (ok) {
+      dims = (int)PyTuple_GET_SIZE(shape);
+      for (int i = 0; i < dims && i < 4; ++i) {
+        n[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+        by[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(steps, i));
+      }
+    }
+    Py_DECREF(shape);
+    Py_XDECREF(steps);
+    if (PyErr_Occurred()) return false;
+    if (!ok || dims > 4) return fail(PyExc_ValueError, "a tensor with up to four dimensions is expected");
+    if (count() > 0) {
+      PyObject* p = PyObject_CallMethodNoArgs(o, s_data_ptr);
+      if (!p) return false;
+      ptr = PyLong_AsVoidPtr(p);
+      Py_DECREF(p);
+      if (PyErr_Occurred()) return false;
+    }
+    return true;
+  }
+  bool has_type(int t) const { return type == t || fail(PyExc_TypeError, t == PSKV_F32 ? "float32 is expected" : "int32 is expected"); }
+  bool is_rows_type() const {
+    return type == PSKV_F32 || type == PSKV_F16 || type == PSKV_BF16 || fail(PyExc_TypeError, "float32, float16 or bfloat16 is expected");
+  }
+  bool dense() const {
+    int64_t want = 1;
+    for (int d = dims; d-- > 0;) {
+      if (n[d] > 1 && by[d] != want && count() > 0) return fail(PyExc_ValueError, "the tensor is not contiguous");
+      want *= n[d];
+    }
+    return true;
+  }
+  // [n, k] with the elements of a row side by side
+  bool is_matrix() const {
+    if (dims != 2) return fail(PyExc_ValueError, "a matrix is expected");
+    if (n[1] > 1 && by[1] != 1 && count() > 0) return fail(PyExc_ValueError, "the elements of a row do not lie side by side");
+    return true;
+  }
+  bool like(const Tensor& o) const {
+    if (type != o.type) return fail(PyExc_TypeError, "not of the type of the other rows");
+    return true;
+  }
+  bool sized(int64_t rows, int64_t k) const {
+    return (dims == 2 && n[0] == rows && n[1] == k) || fail(PyExc_ValueError, "its shape does not fit the other tensors'");
+  }
+};
+
+// All on one device.
+bool together(std::initializer_list<const Tensor*> all, int* device) {
+  *device = -1;
+  for (const Tensor* t : all) {
+    if (!t->given()) continue;
+    if (*device >= 0 && t->device != *device) return t->fail(PyExc_ValueError, "the tensors of a call lie on one device");
+    *device = t->device;
+  }
+  return true;
+}
+
+// The stream of a call: an address, or None for torch's current one on the tensors' device.
+bool stream_of(PyObject* o, int device, void** stream) {
+  if (o != Py_None) {
+    *stream = PyLong_AsVoidPtr(o);
+    return *stream || !PyErr_Occurred();
+  }
+  PyObject* at = PyLong_FromLong(device);
+  PyObject* raw = at ? PyObject_CallOneArg(g_raw_stream, at) : nullptr;
+  Py_XDECREF(at);
+  if (!raw) return false;
+  *stream = PyLong_AsVoidPtr(raw);
+  Py_DECREF(raw);
+  return *stream || !PyErr_Occurred();
+}
+
+#define NEED(x) \
+  do {          \
+    if (!(x)) return nullptr; \
+  } while (0)
+
+// A place of every choice of every token.
+bool is_places(const Tensor& place) {
+  return place.has_type(kInt32) && (place.dims == 2 || place.fail(PyExc_ValueError, "[tokens, choices] is expected")) && place.dense();
+}
+
+// [tokens, choices] of float32
+bool is_weights(const Tensor& w, const Tensor& place) {
+  return w.has_type(PSKV_F32) && w.sized(place.n[0], place.n[1]) && w.dense();
+}
+
+// The working memory of a call: a byte count that it still needs, or 0. -1: refused.
+int64_t working_memory(const Tensor& work, size_t room) {
+  if (!work.given()) return (int64_t)room;
+  if (!work.dense()) return -1;
+  return 0;
+}
+size_t work_bytes(const Tensor& work) {
+  return (size_t)work.count() * (work.type == kInt64 ? 8 : work.type == kInt32 || work.type == PSKV_F32 ? 4 : 2);
+}
+
+// route_sort(experts, E, order, place, offsets, work, stream): a status, or how many bytes of working memory are missing
+PyObject* route_sort(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NEED(want(n, 7));
+  Tensor experts("experts"), order("order"), place("place"), offsets("offsets"), work("work");
+  const size_t E = PyLong_AsSize_t(a[1]);
+  NEED(!PyErr_Occurred());
+  NEED(experts.take(a[0]) && order.take(a[2]) && place.take(a[3]) && offsets.take(a[4]) && work.take(a[5], true));
+  if (experts.type != kInt32 && experts.type != kInt64) NEED(experts.fail(PyExc_TypeError, "int32 or int64 is expected"));
+  NEED(experts.dense() && order.has_type(kInt32) && order.dense() && place.has_type(kInt32) && place.dense() &&
+       offsets.has_type(kInt32) && offsets.dense());
+  const int64_t count = experts.count();
+  if (order.count() != count) NEED(order.fail(PyExc_ValueError, "as many entries as experts has are expected"));
+  if (place.count() != count) NEED(place.fail(PyExc_ValueError, "as many entries as experts has are expected"));
+  if ((uint64_t)offsets.count() != (uint64_t)E + 1) NEED(offsets.fail(PyExc_ValueError, "E + 1 entries are expected"));
+  int device;
+  void* stream;
+  NEED(together({&experts, &order, &place, &offsets, &work}, &device) && stream_of(a[6], device, &stream));
+  const int64_t missing = working_memory(work, pskv_route_room((size_t)count, E));
+  NEED(missing >= 0);
+  if (missing) return PyLong_FromLongLong(missing);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pskv_route_sort(device, stream, experts.ptr, experts.type == kInt64 ? 64 : 32, (size_t)count, E,
+                       static_cast<int32_t*>(order.ptr), static_cast<int32_t*>(place.ptr), static_cast<int32_t*>(offsets.ptr),
+                       work.ptr, work_bytes(work));
+  Py_END_ALLOW_THREADS;
+  return PyLong_FromLong(rc);
+}
+
+// route_rows(x, place, rows, stream)
+PyObject* route_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NEED(want(n, 4));
+  Tensor x("x"), place("place"), rows("rows");
+  NEED(x.take(a[0]) && place.take(a[1]) && rows.take(a[2]) && x.is_rows_type() && x.is_matrix() && is_places(place) &&
+       rows.like(x) && rows.is_matrix() && rows.sized(rows.n[0], x.n[1]));
+  if (place.n[0] != x.n[0]) NEED(place.fail(PyExc_ValueError, "its shape does not fit the other tensors'"));
+  int device, rc;
+  void* stream;
+  NEED(together({&x, &place, &rows}, &device) && stream_of(a[3], device, &stream));
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pskv_route_rows(device, stream, x.type, x.ptr, x.stride(0, x.n[1]), (size_t)x.n[0], (size_t)x.n[1],
+                       static_cast<int32_t*>(place.ptr), (size_t)place.n[1], rows.ptr, rows.stride(0, rows.n[1]), (size_t)rows.n[0]);
+  Py_END_ALLOW_THREADS;
+  return PyLong_FromLong(rc);
+}
+
+// route_sum(rows, place, out, weights, stream)
+PyObject* route_sum(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NEED(want(n, 5));
+  Tensor rows("rows"), place("place"), out("out"), weights("weights");
+  NEED(rows.take(a[0]) && place.take(a[1]) && out.take(a[2]) && weights.take(a[3], true) && rows.is_rows_type() &&
+       rows.is_matrix() && is_places(place) && out.like(rows) && out.is_matrix() && out.sized(place.n[0], rows.n[1]));
+  NEED(!weights.given() || is_weights(weights, place));
+  int device, rc;
+  void* stream;
+  NEED(together({&rows, &place, &out, &weights}, &device) && stream_of(a[4], device, &stream));
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pskv_route_sum(device, stream, rows.type, rows.ptr, rows.stride(0, rows.n[1]), (size_t)rows.n[0],
+                      static_cast<int32_t*>(place.ptr), static_cast<float*>(weights.ptr), (size_t)place.n[1], out.ptr,
+                      out.stride(0, out.n[1]), (size_t)out.n[0], (size_t)out.n[1]);
+  Py_END_ALLOW_THREADS;
+  return PyLong_FromLong(rc);
+}
+
+// route_sum_grad(grad, rows, place, weights, grad_rows, grad_weights, stream)
+PyObject* route_sum_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NEED(want(n, 7));
+  Tensor grad("grad"), rows("rows"), place("place"), weights("weights"), grad_rows("grad_rows"), grad_weights("grad_weights");
+  NEED(grad.take(a[0]) && rows.take(a[1]) && place.take(a[2]) && weights.take(a[3]) && grad_rows.take(a[4]) &&
+       grad_weights.take(a[5]));
+  NEED(grad.is_rows_type() && grad.is_matrix() && is_places(place) && is_weights(weights, place) &&
+       is_weights(grad_weights, place) && rows.like(grad) && rows.is_matrix() && grad_rows.like(grad) && grad_rows.is_matrix() &&
+       rows.sized(rows.n[0], grad.n[1]) && grad_rows.sized(rows.n[0], grad.n[1]) && grad.sized(place.n[0], grad.n[1]));
+  int device, rc;
+  void* stream;
+  NEED(together({&grad, &rows, &place, &weights, &grad_rows, &grad_weights}, &device) && stream_of(a[6], device, &stream));
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pskv_route_sum_grad(device, stream, grad.type, grad.ptr, grad.stride(0, grad.n[1]), (size_t)grad.n[0], (size_t)grad.n[1],
+                           rows.ptr, rows.stride(0, rows.n[1]), (size_t)rows.n[0], static_cast<int32_t*>(place.ptr),
+                           static_cast<float*>(weights.ptr), (size_t)place.n[1], grad_rows.ptr,
+                           grad_rows.stride(0, grad_rows.n[1]), static_cast<float*>(grad_weights.ptr));
+  Py_END_ALLOW_THREADS;
+  return PyLong_FromLong(rc);
+}
+
+// [batch, heads, queries, keys], or without the batch
+struct Scores {
+  size_t n[4];
+  int64_t by[3];
+  bool parse(const Tensor& t) {
+    if (t.dims != 3 && t.dims != 4) return t.fail(PyExc_ValueError, "[heads, queries, keys] with or without a batch is expected");
+    const int o = t.dims - 4;
+    for (int d = 0; d < 4; ++d) n[d] = d + o < 0 ? 1 : (size_t)t.n[d + o];
+    for (int d = 0; d < 3; ++d) by[d] = d + o < 0 || t.n[d + o] < 2 ? 0 : t.by[d + o];
+    if (n[3] > 1 && t.by[3 + o] != 1 && t.count() > 0) return t.fail(PyExc_ValueError, "the keys of a query do not lie side by side");
+    return true;
+  }
+};
+
+bool is_positions(const Tensor& at, size_t batch) {
+  if (!at.given()) return true;
+  if (at.type != kInt64) return at.fail(PyExc_TypeError, "int64 is expected");
+  if (at.dims != 1 || (size_t)at.n[0] != batch) return at.fail(PyExc_ValueError, "a position for each of the batch is expected");
+  return at.dense();
+}
+
+// relbias(table, out, max_distance, two_sided, scores, q_first, k_first, q_at, stream)
+PyObject* relbias(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NEED(want(n, 9));
+  Tensor table("table"), out("out"), scores("scores"), at("q_at");
+  const uint64_t far = PyLong_AsUnsignedLongLong(a[2]);
+  NEED(!PyErr_Occurred());
+  const int two_sided = PyObject_IsTrue(a[3]);
+  const long long q_first = PyLong_AsLongLong(a[5]), k_first = PyLong_AsLongLong(a[6]);
+  NEED(!PyErr_Occurred());
+  NEED(table.take(a[0]) && out.take(a[1]) && scores.take(a[4], true) && at.take(a[7], true) && table.has_type(PSKV_F32) &&
+       table.dense() && out.is_rows_type());
+  if (table.dims != 2) NEED(table.fail(PyExc_ValueError, "[buckets, heads] is expected"));
+  Scores o, s{};
+  NEED(o.parse(out) && is_positions(at, o.n[0]));
+  if ((size_t)table.n[1] != o.n[1]) NEED(table.fail(PyExc_ValueError, "a column for each head is expected"));
+  if (scores.given()) {
+    NEED(scores.like(out) && s.parse(scores));
+    bool same = scores.dims == out.dims;
+    for (int d = 0; d < 4; ++d) same = same && s.n[d] == o.n[d];
+    if (!same) NEED(scores.fail(PyExc_ValueError, "the shape of out is expected"));
+  }
+  int device, rc;
+  void* stream;
+  NEED(together({&table, &out, &scores, &at}, &device) && stream_of(a[8], device, &stream));
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pskv_relbias(device, stream, out.type, static_cast<float*>(table.ptr), (size_t)table.n[0], o.n[1], far, two_sided, q_first,
+                    k_first, static_cast<int64_t*>(at.ptr), scores.ptr, s.by, out.ptr, o.by, o.n[0], o.n[2], o.n[3]);
+  Py_END_ALLOW_THREADS;
+  return PyLong_FromLong(rc);
+}
+
+// relbias_grad(grad, grad_table, max_distance, two_sided, q_first, k_first, q_at, work, stream): as route_sort
+PyObject* relbias_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NEED(want(n, 9));
+  Tensor grad("grad"), grad_table("grad_table"), at("q_at"), work("work");
+  const uint64_t far = PyLong_AsUnsignedLongLong(a[2]);
+  NEED(!PyErr_Occurred());
+  const int two_sided = PyObject_IsTrue(a[3]);
+  const long long q_first = PyLong_AsLongLong(a[4]), k_first = PyLong_AsLongLong(a[5]);
+  NEED(!PyErr_Occurred());
+  NEED(grad.take(a[0]) && grad_table.take(a[1]) && at.take(a[6], true) && work.take(a[7], true) && grad.is_rows_type() &&
+       grad_table.has_type(PSKV_F32) && grad_table.dense());
+  Scores g;
+  NEED(g.parse(grad) && is_positions(at, g.n[0]));
+  if (grad_table.dims != 2 || (size_t)grad_table.n[1] != g.n[1])
+    NEED(grad_table.fail(PyExc_ValueError, "[buckets, heads] is expected"));
+  int device, rc;
+  void* stream;
+  NEED(together({&grad, &grad_table, &at, &work}, &device) && stream_of(a[8], device, &stream));
+  const size_t buckets = (size_t)grad_table.n[0];
+  const int64_t missing =
+      working_memory(work, pskv_relbias_grad_room(buckets, g.n[1], g.n[0], g.n[2], g.n[3], at.given() ? 1 : 0));
+  NEED(missing >= 0);
+  if (missing) return PyLong_FromLongLong(missing);
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pskv_relbias_grad(device, stream, grad.type, grad.ptr, g.by, buckets, g.n[1], far, two_sided, q_first, k_first,
+                         static_cast<int64_t*>(at.ptr), g.n[0], g.n[2], g.n[3], static_cast<float*>(grad_table.ptr), work.ptr,
+                         work_bytes(work));
+  Py_END_ALLOW_THREADS;
+  return PyLong_FromLong(rc);
+}
+
+// dropout(x, out, p, seed, step, keys, first, stream)
+PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  NEED(want(n, 8));
+  Tensor x("x"), out("out"), step("step"), keys("keys");
+  const double p = PyFloat_AsDouble(a[2]);
+  NEED(!PyErr_Occurred());
+  const uint64_t seed = PyLong_AsUnsignedLongLong(a[3]);
+  NEED(!PyErr_Occurred());
+  const uint64_t first = PyLong_AsUnsignedLongLong(a[6]);
+  NEED(!PyErr_Occurred());
+  NEED(x.take(a[0]) && out.take(a[1]) && step.take(a[4], true) && keys.take(a[5], true) && x.is_rows_type() && x.is_matrix() &&
+       out.like(x) && out.is_matrix() && out.sized(x.n[0], x.n[1]));
+  if (step.given() && (step.type != kInt64 || step.count() != 1)) NEED(step.fail(PyExc_TypeError, "one word of 64 bits is expected"));
+  if (keys.given()) {
+    if (keys.type != kInt64) NEED(keys.fail(PyExc_TypeError, "keys of 64 bits are expected"));
+    if (keys.count() != x.n[0]) NEED(keys.fail(PyExc_ValueError, "a key for each row is expected"));
+    NEED(keys.dense());
+  }
+  int device, rc;
+  void* stream;
+  NEED(together({&x, &out, &step, &keys}, &device) && stream_of(a[7], device, &stream));
+  Py_BEGIN_ALLOW_THREADS;
+  rc = pskv_dropout(device, stream, x.type, x.ptr, x.stride(0, x.n[1]), out.ptr, out.stride(0, out.n[1]), (size_t)x.n[0],
+                    (size_t)x.n[1], p, seed, static_cast<uint64_t*>(step.ptr), static_cast<uint64_t*>(keys.ptr), first);
+  Py_END_ALLOW_THREADS;
+  return PyLong_FromLong(rc);
+}
+
+// setup(tensor_type, int64, uint64, float32, int32, raw_stream, float16, bfloat16)
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (!want(n, 6)) return nullptr;
-  PyObject** to[6] = {&g_tensor_type, &g_int64, &g_uint64, &g_float32, &g_int32, &g_raw_stream};
-  for (int i = 0; i < 6; ++i) {
+  if (!want(n, 8)) return nullptr;
+  PyObject** to[8] = {&g_tensor_type, &g_int64, &g_uint64, &g_float32, &g_int32, &g_raw_stream, &g_float16, &g_bfloat16};
+  for (int i = 0; i < 8; ++i) {
     Py_INCREF(a[i]);
     Py_XDECREF(*to[i]);
     *to[i] = a[i];
@@ -383,7 +724,9 @@ PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(setup),      FAST(table_push), FAST(table_pull),     FAST(table_pushpull),
                          FAST(group_push), FAST(group_pull), FAST(group_pushpull), FAST(slice),
-                         FAST(match),      {"replay_run", replay_run, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                         FAST(match),      FAST(route_sort), FAST(route_rows),     FAST(route_sum),
+                         FAST(route_sum_grad), FAST(relbias), FAST(relbias_grad),  FAST(dropout),
+                         {"replay_run", replay_run, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -395,6 +738,9 @@ PyMODINIT_FUNC PyInit__native(void) {
   s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
   s_numel = PyUnicode_InternFromString("numel");
   s_data_ptr = PyUnicode_InternFromString("data_ptr");
-  if (!s_dtype || !s_is_cuda || !s_is_contiguous || !s_numel || !s_data_ptr) return nullptr;
+  s_shape = PyUnicode_InternFromString("shape");
+  s_stride = PyUnicode_InternFromString("stride");
+  s_get_device = PyUnicode_InternFromString("get_device");
+  if (!s_dtype || !s_is_cuda || !s_is_contiguous || !s_numel || !s_data_ptr || !s_shape || !s_stride || !s_get_device) return nullptr;
   return PyModule_Create(&module);
 }

@@ -1,0 +1,445 @@
+// Tokens to the experts they chose, and back (gfx950). T tokens name K experts each; choice i = t*K + j. The choices are
+// sorted by expert, stably, so that every expert finds its rows back to back; a token's row is copied to its K places, and the
+// experts' answers come back as a weighted sum:
+//     place[i]      = #{choices of lower experts} + #{earlier choices of the same expert}
+//     rows[place]   = x[t]                              its gradient: dx[t] = sum_j drows[place[t,j]]
+//     y[t]          = sum_j w[t,j] answers[place[t,j]]  its gradient: danswers[place] = w dy[t], dw[t,j] = <dy[t], answers[place]>
+// Everything but the sort goes token by token: a token's own row is read or written once, its K others once each, nothing is
+// summed by more than one wavefront, and no sum depends on the order in which workgroups run.
+#include <hip/hip_runtime.h>
+
+#include "host_common.h"
+#include "row_types.h"
+
+namespace pskv {
+namespace {
+
+// --- sorting by expert -------------------------------------------------------------------------------------------
+
+constexpr unsigned kSortBlock = 1024;
+constexpr unsigned kSortWaves = kSortBlock / 64;
+constexpr unsigned kSortItems = 8;  // choices per lane
+constexpr unsigned kSortTile = kSortBlock * kSortItems;
+// Up to so many tiles, every workgroup adds up the tiles' counts for itself; beyond, a launch of its own does.
+constexpr unsigned kSortFew = 32;
+constexpr unsigned kSortBins = PSKV_ROUTE_MAX_EXPERTS + 1;  // the last one in use: choices that are not here
+
+template <typename I>
+__device__ __forceinline__ unsigned bin_of(const I* experts, uint64_t i, unsigned E) {
+  const I e = experts[i];
+  return e >= 0 && e < (I)E ? (unsigned)e : E;
+}
+
+// How many choices of every bin a tile has: counts[tile][bin].
+template <typename I>
+__global__ __launch_bounds__(kSortBlock) void k_route_count(const I* __restrict__ experts, uint64_t n, unsigned E,
+                                                             unsigned* __restrict__ counts) {
+  __shared__ unsigned hist[kSortBins];
+  for (unsigned e = threadIdx.x; e <= E; e += kSortBlock) hist[e] = 0;
+  __syncthreads();
+  const uint64_t first = (uint64_t)blockIdx.x * kSortTile;
+#pragma unroll
+  for (unsigned s = 0; s < kSortItems; ++s) {
+    const uint64_t i = first + s * kSortBlock + threadIdx.x;
+    if (i < n) atomicAdd(&hist[bin_of(experts, i, E)], 1u);
+  }
+  __syncthreads();
+  for (unsigned e = threadIdx.x; e <= E; e += kSortBlock) counts[(uint64_t)blockIdx.x * (E + 1) + e] = hist[e];
+}
+
+// What every tile's choices of a bin follow, in place, and behind the last tile the bins' totals. A thread per bin, which
+// reads ahead: the tiles' counts do not depend on each other.
+__global__ __launch_bounds__(64) void k_route_scan(unsigned* __restrict__ counts, unsigned tiles, unsigned bins) {
+  const unsigned e = blockIdx.x * 64 + threadIdx.x;
+  if (e >= bins) return;
+  constexpr unsigned kAhead = 16;
+  unsigned run = 0;
+  for (unsigned t0 = 0; t0 < tiles; t0 += kAhead) {
+    unsigned c[kAhead];
+#pragma unroll
+    for (unsigned a = 0; a < kAhead; ++a) c[a] = t0 + a < tiles ? counts[(uint64_t)(t0 + a) * bins + e] : 0;
+#pragma unroll
+    for (unsigned a = 0; a < kAhead; ++a) {
+      if (t0 + a < tiles) counts[(uint64_t)(t0 + a) * bins + e] = run;
+      run += c[a];
+    }
+  }
+  counts[(uint64_t)tiles * bins + e] = run;
+}
+
+// Places of a tile's choices. A wavefront owns 512 neighbouring ones and takes them 64 at a time: lanes of the same bin find
+// each other by comparing the bits of their bins, so a choice's rank among its wavefront's is known without atomics; ranks
+// begin where the earlier wavefronts', tiles' and bins' choices end.
+template <typename I>
+__global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict__ experts, uint64_t n, unsigned E,
+                                                             const unsigned* __restrict__ counts, unsigned tiles,
+                                                             bool scanned, int* __restrict__ order, int* __restrict__ place,
+                                                             int* __restrict__ offsets) {
+  __shared__ unsigned short mine[kSortWaves][kSortBins];  // of a wavefront, then of those before it
+  __shared__ unsigned base[kSortBins];
+  __shared__ unsigned sums[kSortWaves];
+  const unsigned bins = E + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (unsigned e = lane; e < bins; e += 64) mine[wave][e] = 0;
+  const uint64_t first = (uint64_t)blockIdx.x * kSortTile + wave * (64 * kSortItems) + lane;
+  unsigned bin[kSortItems], rank[kSortItems];
+#pragma unroll
+  for (unsigned s = 0; s < kSortItems; ++s) bin[s] = first + s * 64 < n ? bin_of(experts, first + s * 64, E) : bins;
+  const unsigned bits = 32 - __builtin_clz(bins);
+  const uint64_t before = (1ull << lane) - 1;
+#pragma unroll
+  for (unsigned s = 0; s < kSortItems; ++s) {
+    uint64_t same = ~0ull;
+    for (unsigned b = 0; b < bits; ++b) {
+      const bool one = (bin[s] >> b) & 1;
+      const uint64_t ones = __ballot(one);
+      same &= one ? ones : ~ones;
+    }
+    if (bin[s] < bins) {
+      const unsigned so_far = mine[wave][bin[s]];
+      rank[s] = so_far + __popcll(same & before);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if ((same >> lane) == 1) mine[wave][bin[s]] = (unsigned short)(so_far + __popcll(same));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  __syncthreads();
+  // where every bin begins: its own total over all tiles, summed up over the bins, four to a thread
+  constexpr unsigned kPer = (kSortBins + kSortBlock - 1) / kSortBlock;
+  unsigned total[kPer], earlier[kPer], all = 0;
+#pragma unroll
+  for (unsigned q = 0; q < kPer; ++q) {
+    const unsigned e = threadIdx.x * kPer + q;
+    total[q] = earlier[q] = 0;
+    if (e < bins) {
+      unsigned run = 0;
+      for (unsigned w = 0; w < kSortWaves; ++w) {
+        const unsigned c = mine[w][e];
+        mine[w][e] = (unsigned short)run;
+        run += c;
+      }
+      total[q] = run;
+      if (scanned) {
+        total[q] = counts[(uint64_t)tiles * bins + e];
+        earlier[q] = counts[(uint64_t)blockIdx.x * bins + e];
+      } else if (tiles > 1) {
+        total[q] = 0;
+        for (unsigned t = 0; t < tiles; ++t) {
+          const unsigned c = counts[(uint64_t)t * bins + e];
+          total[q] += c;
+          earlier[q] += t < blockIdx.x ? c : 0;
+        }
+      }
+    }
+    all += total[q];
+  }
+  unsigned inc = all;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned up = __shfl_up(inc, o);
+    inc += lane >= (unsigned)o ? up : 0;
+  }
+  if (lane == 63) sums[wave] = inc;
+  __syncthreads();
+  unsigned run = inc - all;
+  for (unsigned w = 0; w < wave; ++w) run += sums[w];
+#pragma unroll
+  for (unsigned q = 0; q < kPer; ++q) {
+    const unsigned e = threadIdx.x * kPer + q;
+    if (e < bins) {
+      base[e] = run + earlier[q];
+      if (blockIdx.x == 0) offsets[e] = (int)run;
+    }
+    run += total[q];
+  }
+  __syncthreads();
+#pragma unroll
+  for (unsigned s = 0; s < kSortItems; ++s) {
+    if (bin[s] >= bins) continue;
+    const uint64_t i = first + s * 64;
+    const unsigned p = base[bin[s]] + mine[wave][bin[s]] + rank[s];
+    const bool here = bin[s] < E;
+    place[i] = here ? (int)p : -1;
+    order[p] = here ? (int)i : -1;
+  }
+}
+
+// --- rows out and back -------------------------------------------------------------------------------------------
+
+constexpr unsigned kRowBlock = 256;
+
+struct RowArgs {
+  uint64_t tokens, k, rows;      // rows: of the sorted side
+  uint64_t token_stride, row_stride;  // elements
+  unsigned choices, lanes_log2;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ x, const int* __restrict__ place,
+                                                           T* __restrict__ out, RowArgs a) {
+  using Vec = typename Row<T>::Vec;
+  constexpr unsigned W = Row<T>::kWide;
+  const unsigned lanes = 1u << a.lanes_log2;
+  const uint64_t per = (uint64_t)gridDim.x * (kRowBlock >> a.lanes_log2);
+  for (uint64_t t = ((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2; t < a.tokens; t += per) {
+    const T* from = x + t * a.token_stride;
+    const int* at = place + t * a.choices;
+    for (uint64_t c = (uint64_t)(threadIdx.x & (lanes - 1)) * W; c < a.k; c += (uint64_t)lanes * W) {
+      if (c + W <= a.k) {
+        const Vec v = *reinterpret_cast<const Vec*>(from + c);
+        for (unsigned j = 0; j < a.choices; ++j) {
+          const uint64_t p = (uint64_t)(int64_t)at[j];
+          if (p < a.rows) *reinterpret_cast<Vec*>(out + p * a.row_stride + c) = v;
+        }
+      } else {
+        for (unsigned j = 0; j < a.choices; ++j) {
+          const uint64_t p = (uint64_t)(int64_t)at[j];
+          if (p < a.rows)
+            for (uint64_t i = c; i < a.k; ++i) out[p * a.row_stride + i] = from[i];
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ rows, const int* __restrict__ place,
+                                                          const float* __restrict__ weights, T* __restrict__ out, RowArgs a) {
+  using Vec = typename Row<T>::Vec;
+  constexpr unsigned W = Row<T>::kWide;
+  const unsigned lanes = 1u << a.lanes_log2;
+  const uint64_t per = (uint64_t)gridDim.x * (kRowBlock >> a.lanes_log2);
+  for (uint64_t t = ((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2; t < a.tokens; t += per) {
+    const int* at = place + t * a.choices;
+    const float* w = weights ? weights + t * a.choices : nullptr;
+    T* to = out + t * a.token_stride;
+    for (uint64_t c = (uint64_t)(threadIdx.x & (lanes - 1)) * W; c < a.k; c += (uint64_t)lanes * W) {
+      const unsigned wide = c + W <= a.k ? W : (unsigned)(a.k - c);
+      float sum[W] = {};
+      for (unsigned j = 0; j < a.choices; ++j) {
+        const uint64_t p = (uint64_t)(int64_t)at[j];
+        if (p >= a.rows) continue;
+        const float f = w ? w[j] : 1.0f;
+        const T* from = rows + p * a.row_stride + c;
+        if (wide == W) {
+          const Vec v = *reinterpret_cast<const Vec*>(from);
+  #pragma unroll
+          for (unsigned i = 0; i < W; ++i) sum[i] = __builtin_fmaf(f, (float)v[i], sum[i]);
+        } else {
+  #pragma unroll
+          for (unsigned i = 0; i < W; ++i)
+            if (i < wide) sum[i] = __builtin_fmaf(f, (float)from[i], sum[i]);
+        }
+      }
+      if (wide == W) {
+        Vec v;
+  #pragma unroll
+        for (unsigned i = 0; i < W; ++i) v[i] = (T)sum[i];
+        *reinterpret_cast<Vec*>(to + c) = v;
+      } else {
+  #pragma unroll
+        for (unsigned i = 0; i < W; ++i)
+          if (i < wide) to[c + i] = (T)sum[i];
+      }
+    }
+  }
+}
+
+// At most a wavefront per token, so that the products' sums need no other than its own lanes.
+template <typename T>
+__global__ __launch_bounds__(kRowBlock) void k_route_sum_grad(const T* __restrict__ grad, const T* __restrict__ rows,
+                                                               const int* __restrict__ place,
+                                                               const float* __restrict__ weights, T* __restrict__ grad_rows,
+                                                               uint64_t grad_row_stride, float* __restrict__ grad_weights,
+                                                               RowArgs a) {
+  using Vec = typename Row<T>::Vec;
+  constexpr unsigned W = Row<T>::kWide;
+  const unsigned lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1), own = threadIdx.x >> a.lanes_log2;
+  const uint64_t per = kRowBlock >> a.lanes_log2;
+  for (uint64_t t0 = blockIdx.x * per; t0 < a.tokens; t0 += gridDim.x * per) {
+    const uint64_t t = t0 + own;
+    const bool is = t < a.tokens;  // (no lane leaves: they add up together)
+    const T* g = grad + t * a.token_stride;
+    for (unsigned j = 0; j < a.choices; ++j) {
+      const uint64_t p = is ? (uint64_t)(int64_t)place[t * a.choices + j] : ~0ull;
+      float sum = 0.0f;
+      if (p < a.rows) {
+        const float f = weights[t * a.choices + j];
+        const T* from = rows + p * a.row_stride;
+        T* to = grad_rows + p * grad_row_stride;
+        for (uint64_t c = (uint64_t)lane * W; c < a.k; c += (uint64_t)lanes * W) {
+          if (c + W <= a.k) {
+            const Vec d = *reinterpret_cast<const Vec*>(g + c), v = *reinterpret_cast<const Vec*>(from + c);
+            Vec o;
+  #pragma unroll
+            for (unsigned i = 0; i < W; ++i) {
+              sum = __builtin_fmaf((float)d[i], (float)v[i], sum);
+              o[i] = (T)(f * (float)d[i]);
+            }
+            *reinterpret_cast<Vec*>(to + c) = o;
+          } else {
+            for (uint64_t i = c; i < a.k; ++i) {
+              sum = __builtin_fmaf((float)g[i], (float)from[i], sum);
+              to[i] = (T)(f * (float)g[i]);
+            }
+          }
+        }
+      }
+      for (unsigned o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+      if (is && lane == 0) grad_weights[t * a.choices + j] = sum;
+    }
+  }
+}
+
+// --- the host's checks -------------------------------------------------------------------------------------------
+
+// What every call between tokens and sorted rows refuses. PSKV_OK: it may run.
+int check_rows(int type, uint64_t tokens, uint64_t choices, uint64_t rows, uint64_t k) {
+  if (!type_bytes(type)) return set_error(PSKV_EINVAL, "type %d: PSKV_F32, PSKV_F16 or PSKV_BF16", type);
+  if (choices == 0) return set_error(PSKV_EINVAL, "a token chooses at least one expert");
+  if (k == 0 || k > (1ull << 30)) return set_error(PSKV_EINVAL, "rows of 1 to 2^30 elements");
+  if (tokens > 0x7fffffffull || choices > 0x7fffffffull || tokens * choices > 0x7fffffffull || rows > 0x7fffffffull)
+    return set_error(PSKV_EINVAL, "2^31 - 1 choices and rows at most");
+  return PSKV_OK;
+}
+
+int check_stride(const char* what, uint64_t n, uint64_t k, uint64_t stride, bool written) {
+  if (stride > (1ull << 40)) return set_error(PSKV_EINVAL, "%s: rows 2^40 elements apart at most", what);
+  if (written && n > 1 && stride < k) return set_error(PSKV_EINVAL, "%s: rows that are written lie upon each other", what);
+  return PSKV_OK;
+}
+
+unsigned row_grid(uint64_t tokens, unsigned lanes_log2) {
+  return grid_for(tokens, kRowBlock >> lanes_log2, 1u << 22);
+}
+
+RowArgs row_args(uint64_t tokens, uint64_t choices, uint64_t rows, uint64_t k, uint64_t token_stride, uint64_t row_stride,
+                 int type, unsigned most_lanes) {
+  const uint64_t wide = 16 / type_bytes(type);
+  const unsigned lanes = lanes_for((k + wide - 1) / wide, most_lanes);
+  return RowArgs{tokens, k, rows, token_stride, row_stride, (unsigned)choices, (unsigned)__builtin_ctz(lanes)};
+}
+
+}  // namespace
+}  // namespace pskv
+
+using namespace pskv;
+
+#define RETURN_IF(call)     \
+  do {                      \
+    const int rc_ = (call); \
+    if (rc_) return rc_;    \
+  } while (0)
+
+extern "C" size_t pskv_route_room(size_t n, size_t E) {
+  if (n <= kSortTile || n > 0x7fffffffull || E > PSKV_ROUTE_MAX_EXPERTS) return 0;
+  return ((n + kSortTile - 1) / kSortTile + 1) * (E + 1) * sizeof(unsigned);
+}
+
+extern "C" int pskv_route_sort(int device, void* stream, const void* experts, int index_bits, size_t n, size_t E,
+                               int32_t* order, int32_t* place, int32_t* offsets, void* work, size_t work_bytes) {
+  clear_error();
+  if (index_bits != 32 && index_bits != 64) return set_error(PSKV_EINVAL, "experts are numbers of 32 or 64 bits");
+  if (E == 0 || E > PSKV_ROUTE_MAX_EXPERTS)
+    return set_error(PSKV_EINVAL, "%zu experts: 1 to %d", E, PSKV_ROUTE_MAX_EXPERTS);
+  if (n > 0x7fffffffull) return set_error(PSKV_EINVAL, "2^31 - 1 choices at most");
+  if (!offsets || (n && (!experts || !order || !place))) return set_error(PSKV_EINVAL, "null buffer");
+  const size_t room = pskv_route_room(n, E);
+  if (room && (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3)))
+    return set_error(PSKV_EINVAL, "a sort of %zu choices takes %zu bytes of working memory, %zu given", n, room,
+                     work ? work_bytes : (size_t)0);
+  DeviceGuard guard(device);
+  if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const unsigned tiles = n <= kSortTile ? 1u : (unsigned)((n + kSortTile - 1) / kSortTile);
+  const bool scanned = tiles > kSortFew;
+  unsigned* counts = static_cast<unsigned*>(work);
+  auto go = [&](auto* e) {
+    using I = std::remove_const_t<std::remove_pointer_t<decltype(e)>>;
+    if (tiles > 1) hipLaunchKernelGGL(k_route_count<I>, dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts);
+    if (scanned) hipLaunchKernelGGL(k_route_scan, dim3((unsigned)E / 64 + 1), dim3(64), 0, st, counts, tiles, (unsigned)E + 1);
+    hipLaunchKernelGGL(k_route_place<I>, dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts, tiles, scanned,
+                       order, place, offsets);
+  };
+  if (index_bits == 64)
+    go(static_cast<const int64_t*>(experts));
+  else
+    go(static_cast<const int32_t*>(experts));
+  PSKV_HIP(hipGetLastError());
+  return PSKV_OK;
+}
+
+extern "C" int pskv_route_rows(int device, void* stream, int type, const void* x, size_t x_stride, size_t tokens, size_t k,
+                               const int32_t* place, size_t choices, void* rows, size_t rows_stride, size_t n_rows) {
+  clear_error();
+  RETURN_IF(check_rows(type, tokens, choices, n_rows, k));
+  RETURN_IF(check_stride("x", tokens, k, x_stride, false));
+  RETURN_IF(check_stride("rows", n_rows, k, rows_stride, true));
+  if (tokens == 0 || n_rows == 0) return PSKV_OK;
+  if (!x || !place || !rows) return set_error(PSKV_EINVAL, "null buffer");
+  const size_t size = type_bytes(type);
+  if (rows_overlap({x, tokens, k, x_stride, size}, {rows, n_rows, k, rows_stride, size}))
+    return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
+  DeviceGuard guard(device);
+  if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
+  const RowArgs a = row_args(tokens, choices, n_rows, k, x_stride, rows_stride, type, kRowBlock);
+  with_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL(k_route_rows<T>, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const T*>(x), place, static_cast<T*>(rows), a);
+  });
+  PSKV_HIP(hipGetLastError());
+  return PSKV_OK;
+}
+
+extern "C" int pskv_route_sum(int device, void* stream, int type, const void* rows, size_t rows_stride, size_t n_rows,
+                              const int32_t* place, const float* weights, size_t choices, void* out, size_t out_stride,
+                              size_t tokens, size_t k) {
+  clear_error();
+  RETURN_IF(check_rows(type, tokens, choices, n_rows, k));
+  RETURN_IF(check_stride("rows", n_rows, k, rows_stride, false));
+  RETURN_IF(check_stride("out", tokens, k, out_stride, true));
+  if (tokens == 0) return PSKV_OK;
+  if ((n_rows && !rows) || !place || !out) return set_error(PSKV_EINVAL, "null buffer");
+  const size_t size = type_bytes(type);
+  if (rows_overlap({rows, n_rows, k, rows_stride, size}, {out, tokens, k, out_stride, size}))
+    return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
+  DeviceGuard guard(device);
+  if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
+  const RowArgs a = row_args(tokens, choices, n_rows, k, out_stride, rows_stride, type, kRowBlock);
+  with_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL(k_route_sum<T>, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const T*>(rows), place, weights, static_cast<T*>(out), a);
+  });
+  PSKV_HIP(hipGetLastError());
+  return PSKV_OK;
+}
+
+extern "C" int pskv_route_sum_grad(int device, void* stream, int type, const void* grad, size_t grad_stride, size_t tokens,
+                                   size_t k, const void* rows, size_t rows_stride, size_t n_rows, const int32_t* place,
+                                   const float* weights, size_t choices, void* grad_rows, size_t grad_rows_stride,
+                                   float* grad_weights) {
+  clear_error();
+  RETURN_IF(check_rows(type, tokens, choices, n_rows, k));
+  RETURN_IF(check_stride("grad", tokens, k, grad_stride, false));
+  RETURN_IF(check_stride("rows", n_rows, k, rows_stride, false));
+  RETURN_IF(check_stride("grad_rows", n_rows, k, grad_rows_stride, true));
+  if (tokens == 0) return PSKV_OK;
+  if (!grad || !place || !weights || !grad_weights || (n_rows && (!rows || !grad_rows)))
+    return set_error(PSKV_EINVAL, "null buffer");
+  const size_t size = type_bytes(type);
+  const RowSpan to{grad_rows, n_rows, k, grad_rows_stride, size};
+  if (rows_overlap({grad, tokens, k, grad_stride, size}, to) || rows_overlap({rows, n_rows, k, rows_stride, size}, to))
+    return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
+  DeviceGuard guard(device);
+  if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
+  const RowArgs a = row_args(tokens, choices, n_rows, k, grad_stride, rows_stride, type, 64);
+  with_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL(k_route_sum_grad<T>, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const T*>(grad), static_cast<const T*>(rows), place, weights,
+                       static_cast<T*>(grad_rows), (uint64_t)grad_rows_stride, grad_weights, a);
+  });
+  PSKV_HIP(hipGetLastError());
+  return PSKV_OK;
+}
