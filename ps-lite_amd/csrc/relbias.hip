@@ -1,8 +1,8 @@
 // The learned relative position bias and its gradient (gfx950):
 //     out[b,h,i,j] = scores[b,h,i,j] + table[bucket(rel)][h],  rel = (k_first + j) - (q_first + q_at[b] + i)
 //     dtable[u][h] = sum of grad[b,h,i,j] over the b, i, j whose bucket is u
-// The bias depends on j - i alone, so a tile of R rows and C columns needs R + C - 1 values of it, which are worked out once
-// and kept in LDS; the gradient sums diagonals first, a lane to each, and diagonals into buckets once per workgroup.
+// The bias depends on j - i alone. Both directions go by tiles of a wavefront whose lanes hand values to each other along the
+// diagonals; the gradient's diagonals are summed into buckets once per tile.
 #include <hip/hip_runtime.h>
 
 #include <new>
@@ -15,7 +15,11 @@ namespace pskv {
 namespace {
 
 constexpr unsigned kBlock = 256;
-constexpr unsigned kCols = 1024, kRows = 32;  // a tile of the bias
+constexpr unsigned kWaves = kBlock / 64;
+constexpr unsigned kWide = 8;            // neighbouring columns of a lane
+constexpr unsigned kCols = 64 * kWide;   // of a wavefront
+constexpr unsigned kGroup = 8;           // rows that a wavefront asks for before it uses them
+constexpr unsigned kMostRows = 128;      // of a wavefront
 
 struct Shape {
   uint64_t B, H, Q, K;
@@ -23,87 +27,277 @@ struct Shape {
   uint64_t in[3], out[3];  // strides of batch, head and row
 };
 
+// How a call is cut up: a wavefront takes `rows` rows of kCols columns of one head, for `batches` batches one after the other.
+struct Cut {
+  unsigned rows, batches;
+  unsigned across, strips, chunks;  // how many there are of columns, rows, batches
+  __host__ __device__ uint64_t tiles() const { return (uint64_t)across * strips * chunks; }  // of a head
+};
+
+// Eight neighbouring elements, as they are in memory and as numbers.
+template <typename T>
+struct Eight {
+  static constexpr int kWords = 2 * (int)sizeof(T);
+  uint32_t word[kWords];
+
+  __device__ __forceinline__ void load(const T* p) {
+    typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int q = 0; q < kWords / 4; ++q) {
+      const Quad v = __builtin_bit_cast(Quad, reinterpret_cast<const typename Row<T>::Vec*>(p)[q]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word[4 * q + i] = v[i];
+    }
+  }
+  // n (up to 8) of them, zeros behind them.
+  __device__ __forceinline__ void few(const T* p, unsigned n) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) word[i] = 0;
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i)
+      if (i < n) {
+        if constexpr (sizeof(T) == 4)
+          word[i] = __builtin_bit_cast(uint32_t, p[i]);
+        else
+          word[i / 2] |= (uint32_t)__builtin_bit_cast(unsigned short, p[i]) << (i & 1 ? 16 : 0);
+      }
+  }
+  // The elements from `off` (up to 8) on, zeros behind them: what a lane at the end of a row needs that has loaded the last eight.
+  __device__ __forceinline__ void skip(unsigned off) {
+    constexpr int kHalf = sizeof(T) == 2 ? 1 : 0;
+    if (kHalf) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i)
+        word[i] = __builtin_amdgcn_alignbit(i + 1 < kWords ? word[i + 1] : 0u, word[i], off & 1 ? 16 : 0);
+    }
+#pragma unroll
+    for (int step = 1; step <= kWords; step <<= 1) {
+      const bool now = ((off >> kHalf) & (unsigned)step) != 0;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) word[i] = now ? (i + step < kWords ? word[i + step] : 0u) : word[i];
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (std::is_same<T, float>::value)
+      return __builtin_bit_cast(float, word[i]);
+    else if constexpr (std::is_same<T, __bf16>::value)
+      return __builtin_bit_cast(float, i & 1 ? word[i / 2] & 0xffff0000u : word[i / 2] << 16);
+    else
+      return (float)__builtin_bit_cast(_Float16, (unsigned short)(i & 1 ? word[i / 2] >> 16 : word[i / 2]));
+  }
+};
+
+// Rounds eight numbers and stores the first n of them.
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, const float (&y)[8], unsigned n) {
+  constexpr int kSome = Row<T>::kWide;
+  if (n == 8) {
+#pragma unroll
+    for (int q = 0; q < 8 / kSome; ++q) {
+      typename Row<T>::Vec v;
+#pragma unroll
+      for (int i = 0; i < kSome; ++i) v[i] = (T)y[q * kSome + i];
+      reinterpret_cast<typename Row<T>::Vec*>(p)[q] = v;
+    }
+  } else {
+#pragma unroll
+    for (unsigned i = 0; i < 7; ++i)
+      if (i < n) p[i] = (T)y[i];
+  }
+}
+
+// The lane below's `v`; lane 0 gets `first`.
+__device__ __forceinline__ float from_below(float v, float first) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, first), __builtin_bit_cast(int, v),
+                                                               0x138 /* wave_shr:1 */, 0xf, 0xf, false));
+}
+
+// A lane's part of the rows of a tile: columns c to c + 7, or what there is of them.
+struct Span {
+  uint64_t at;     // where it loads: at c, or the last eight of the row
+  unsigned off;    // how many of those come before c
+  unsigned own;    // columns, 0 to 8
+  bool ends, few;  // the same for the wavefront: the row ends within its columns; it is shorter than a load
+  __device__ __forceinline__ Span(uint64_t c0, unsigned lane, uint64_t K) {
+    const uint64_t c = c0 + lane * kWide;
+    ends = c0 + kCols > K;
+    few = K < kWide;
+    own = c >= K ? 0 : K - c < kWide ? (unsigned)(K - c) : kWide;
+    at = few || own == kWide ? c : K - kWide;
+    off = c - at < kWide ? (unsigned)(c - at) : kWide;
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(Eight<T>& x, const T* row) const {
+    if (few) {
+      x.few(row + at, own);
+      return;
+    }
+    x.load(row + at);
+    if (ends) x.skip(off);
+  }
+};
+
+// The tile of a wavefront.
+struct Tile {
+  uint64_t c0, r0, head, batch0;
+  unsigned rows, batches;
+  __device__ __forceinline__ Tile(uint64_t tile, const Cut& cut, uint64_t B, uint64_t H, uint64_t Q) {
+    c0 = tile % cut.across * kCols;
+    tile /= cut.across;
+    r0 = tile % cut.strips * cut.rows;
+    tile /= cut.strips;
+    head = tile % H;
+    batch0 = tile / H * cut.batches;
+    rows = Q - r0 < cut.rows ? (unsigned)(Q - r0) : cut.rows;
+    batches = B - batch0 < cut.batches ? (unsigned)(B - batch0) : cut.batches;
+  }
+};
+
+// A tile of the bias. Row i's bias is row i - 1's, moved one column to the right, so eight rows further down a lane needs what
+// the lane below had: eight values of a lane's own and eight that it is handed serve eight rows, and nothing is looked up
+// but the tile's first row and, for lane 0, its first column, which waits in LDS.
 template <typename T, bool SCORES>
 __global__ __launch_bounds__(kBlock) void k_relbias(const float* __restrict__ table, const int64_t* __restrict__ q_at,
-                                                     const T* scores, T* out, Shape s, Buckets b) {
-  __shared__ float bias[kRows + kCols];
-  const uint64_t c0 = (uint64_t)blockIdx.x * kCols, r0 = (uint64_t)blockIdx.y * kRows;
-  const unsigned cols = s.K - c0 < kCols ? (unsigned)(s.K - c0) : kCols;
-  const unsigned rows = s.Q - r0 < kRows ? (unsigned)(s.Q - r0) : kRows;
-  for (uint64_t z = blockIdx.z; z < s.B * s.H; z += gridDim.z) {
-    const uint64_t batch = z / s.H, head = z % s.H;
-    // bias[x]: of the diagonal x - (rows - 1) of the tile
-    const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[batch] : 0) + c0 - r0 - (rows - 1);
-    __syncthreads();
-    for (unsigned x = threadIdx.x; x < rows + cols - 1; x += kBlock)
-      bias[x] = table[(uint64_t)bucket_of(b, (int64_t)(rel + x)) * s.H + head];
-    __syncthreads();
-    const T* from = SCORES ? scores + batch * s.in[0] + head * s.in[1] + r0 * s.in[2] + c0 : nullptr;
-    T* to = out + batch * s.out[0] + head * s.out[1] + r0 * s.out[2] + c0;
-    for (unsigned i = 0; i < rows; ++i)
-      for (unsigned j = threadIdx.x; j < cols; j += kBlock) {
-        const float v = bias[j + rows - 1 - i];
-        to[i * s.out[2] + j] = (T)(SCORES ? (float)from[i * s.in[2] + j] + v : v);
-      }
+                                                     const T* scores, T* out, Cut cut, Shape s, Buckets b) {
+  __shared__ float left[kWaves][kMostRows];  // diagonals -1, -2, ... of the wavefront's tile
+  const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint64_t tiles = cut.tiles() * s.H;
+  for (uint64_t tile = (uint64_t)blockIdx.x * kWaves + wave; tile < tiles; tile += (uint64_t)gridDim.x * kWaves) {
+    const Tile t(tile, cut, s.B, s.H, s.Q);
+    const Span span(t.c0, lane, s.K);
+    const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0;
+    auto value = [&](uint64_t r) { return table[(uint64_t)bucket_of(b, (int64_t)r) * s.H + t.head]; };
+    const unsigned reach = (t.rows + kGroup - 1) / kGroup * kGroup;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (unsigned i = lane; i < reach; i += 64) left[wave][i] = value(rel - 1 - i);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float v[kWide], next[kWide];
+#pragma unroll
+    for (unsigned k = 0; k < kWide; ++k) v[k] = value(rel + lane * kWide + k);
+    const T* from = SCORES ? scores + t.batch0 * s.in[0] + t.head * s.in[1] + t.r0 * s.in[2] : nullptr;
+    T* to = out + t.batch0 * s.out[0] + t.head * s.out[1] + t.r0 * s.out[2] + t.c0 + lane * kWide;
+    for (unsigned i = 0; i < t.rows; i += kGroup) {
+#pragma unroll
+      for (unsigned k = 0; k < kWide; ++k) next[k] = from_below(v[k], left[wave][i + kGroup - 1 - k]);
+      auto group = [&](auto whole) {
+        for (unsigned n = 0; n < t.batches; ++n) {
+          Eight<T> x[kGroup];
+#pragma unroll
+          for (unsigned r = 0; r < kGroup; ++r)
+            if (SCORES && (whole || i + r < t.rows)) span.load(x[r], from + n * s.in[0] + (uint64_t)(i + r) * s.in[2]);
+#pragma unroll
+          for (unsigned r = 0; r < kGroup; ++r) {
+            if (!whole && i + r >= t.rows) continue;
+            float y[kWide];
+#pragma unroll
+            for (unsigned k = 0; k < kWide; ++k) {
+              y[k] = k >= r ? v[k - r] : next[kWide + k - r];
+              if (SCORES) y[k] = x[r].at(k) + y[k];
+            }
+            store_eight(to + n * s.out[0] + (uint64_t)(i + r) * s.out[2], y, span.own);
+          }
+        }
+      };
+      if (i + kGroup <= t.rows)
+        group(std::true_type());
+      else
+        group(std::false_type());
+#pragma unroll
+      for (unsigned k = 0; k < kWide; ++k) v[k] = next[k];
+    }
   }
 }
 
 // --- the gradient ------------------------------------------------------------------------------------------------
 
-constexpr unsigned kSumRows = 128;  // rows of a strip
-
-// A strip: kSumRows rows of one head (of all batches, or of one where they are at positions of their own). A workgroup takes 256
-// neighbouring diagonals of it, a lane adds up one diagonal, row by row and batch by batch.
-// partial[head][bucket][workgroup of the head].
+// The same tiles the other way round: rows are summed over the batch, then along the diagonals, which move up one lane every
+// eight rows; those that leave lane 63 and those that are there in the end are summed by bucket, 64 neighbouring diagonals
+// at a time. Every sum has one order. partial[head][bucket][workgroup of the head].
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ grad, const int64_t* __restrict__ q_at,
-                                                          float* __restrict__ partial, unsigned buckets, unsigned slots,
-                                                          unsigned strips, Shape s, Buckets b) {
-  __shared__ float acc[kBlock / 64][kMostBuckets];
-  const uint64_t head = blockIdx.z;
-  const unsigned strip = blockIdx.y % strips;
-  const uint64_t batch0 = q_at ? blockIdx.y / strips : 0, batches = q_at ? 1 : s.B;
-  const uint64_t r0 = (uint64_t)strip * kSumRows;
-  const unsigned rows = s.Q - r0 < kSumRows ? (unsigned)(s.Q - r0) : kSumRows;
+                                                          float* __restrict__ partial, unsigned buckets, Cut cut, Shape s,
+                                                          Buckets b) {
+  __shared__ float diagonal[kWaves][kMostRows + kCols];
+  __shared__ float sums[kWaves][kMostBuckets];
   const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (unsigned u = lane; u < buckets; u += 64) acc[wave][u] = 0.0f;
-  __syncthreads();
-  // column = diag + row within the strip
-  const int64_t diag = (int64_t)((uint64_t)blockIdx.x * kBlock + threadIdx.x) - (int64_t)(rows - 1);
-  float sum = 0.0f;
-  for (uint64_t n = 0; n < batches; ++n) {
-    const T* from = grad + (batch0 + n) * s.in[0] + head * s.in[1] + r0 * s.in[2];
-    float mine = 0.0f;
-#pragma unroll 8
-    for (unsigned i = 0; i < rows; ++i) {
-      const int64_t j = diag + i;
-      if (j >= 0 && j < (int64_t)s.K) mine += (float)from[i * s.in[2] + j];
+  const uint64_t head = blockIdx.y, tile = (uint64_t)blockIdx.x * kWaves + wave;
+  for (unsigned u = lane; u < buckets; u += 64) sums[wave][u] = 0.0f;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (tile < cut.tiles()) {
+    const Tile t(tile, cut, s.B, 1, s.Q);  // (of this head)
+    const Span span(t.c0, lane, s.K);
+    const T* from = grad + t.batch0 * s.in[0] + head * s.in[1] + t.r0 * s.in[2];
+    const unsigned reach = (t.rows + kGroup - 1) / kGroup * kGroup;
+    float high[kWide] = {};  // of the diagonals that begin the group's first row
+    for (unsigned i = 0; i < t.rows; i += kGroup) {
+      float sum[kGroup][kWide] = {};
+      auto group = [&](auto whole) {
+        for (unsigned n = 0; n < t.batches; ++n) {
+          Eight<T> x[kGroup];
+#pragma unroll
+          for (unsigned r = 0; r < kGroup; ++r)
+            if (whole || i + r < t.rows) span.load(x[r], from + n * s.in[0] + (uint64_t)(i + r) * s.in[2]);
+#pragma unroll
+          for (unsigned r = 0; r < kGroup; ++r)
+            if (whole || i + r < t.rows)
+#pragma unroll
+              for (unsigned k = 0; k < kWide; ++k) sum[r][k] += x[r].at(k);
+        }
+      };
+      if (i + kGroup <= t.rows)
+        group(std::true_type());
+      else
+        group(std::false_type());
+      float low[kWide] = {};
+#pragma unroll
+      for (unsigned r = 0; r < kGroup; ++r)
+#pragma unroll
+        for (unsigned k = 0; k < kWide; ++k) {
+          if (k >= r)
+            high[k - r] += sum[r][k];
+          else
+            low[kWide + k - r] += sum[r][k];
+        }
+#pragma unroll
+      for (unsigned k = 0; k < kWide; ++k) {
+        if (lane == 63) diagonal[wave][kCols - kWide + reach - i + k] = high[k];
+        high[k] = low[k] + from_below(high[k], 0.0f);
+      }
     }
-    sum += mine;
-  }
-  const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[batch0] : 0) + (uint64_t)diag - r0;
-  const unsigned u = diag < (int64_t)s.K ? bucket_of(b, (int64_t)rel) : kMostBuckets;
-  // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
-  unsigned start = __shfl_up(u, 1) != u || lane == 0 ? lane : 0;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned up = __shfl_up(start, o);
-    if (lane >= (unsigned)o && up > start) start = up;
-  }
+    for (unsigned k = 0; k < kWide; ++k) diagonal[wave][lane * kWide + k] = high[k];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // diagonal[x] is the one that is x - reach columns to the right of the tile's corner
+    const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0 - reach;
+    for (unsigned x0 = 0; x0 < reach + kCols; x0 += 64) {
+      const unsigned x = x0 + lane;
+      float sum = x < reach + kCols ? diagonal[wave][x] : 0.0f;
+      const unsigned u = bucket_of(b, (int64_t)(rel + x));
+      // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
+      const unsigned below = __shfl_up(u, 1), above = __shfl_down(u, 1);
+      unsigned start = below != u && lane > 0 ? lane : 0;
+      if (__any(start != 0)) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const float up = __shfl_up(sum, o);
-    if (lane >= start + o) sum += up;
+        for (int o = 1; o < 64; o <<= 1) {
+          const unsigned up = __shfl_up(start, o);
+          if (lane >= (unsigned)o && up > start) start = up;
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const float up = __shfl_up(sum, o);
+        if (lane >= start + o) sum += up;
+      }
+      if (lane == 63 || above != u) sums[wave][u] += sum;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
   }
-  const unsigned next = __shfl_down(u, 1);
-  if (u < buckets && (lane == 63 || next != u)) acc[wave][u] = sum;
   __syncthreads();
-  const unsigned slot = blockIdx.y * gridDim.x + blockIdx.x;
-  for (unsigned v = threadIdx.x; v < buckets; v += kBlock) {
-    float t = acc[0][v];
+  for (unsigned u = threadIdx.x; u < buckets; u += kBlock) {
+    float sum = sums[0][u];
 #pragma unroll
-    for (unsigned w = 1; w < kBlock / 64; ++w) t += acc[w][v];
-    partial[(head * buckets + v) * slots + slot] = t;
+    for (unsigned w = 1; w < kWaves; ++w) sum += sums[w][u];
+    partial[(head * buckets + u) * gridDim.x + blockIdx.x] = sum;
   }
 }
 
@@ -179,16 +373,32 @@ int check_strides(const char* what, const int64_t* stride, const Shape& s, bool 
   return PSKV_OK;
 }
 
-struct SumPlan {
-  unsigned across, strips, down, slots;
-  SumPlan(size_t B, size_t Q, size_t K, bool own_positions) {
-    const size_t rows = Q < kSumRows ? Q : kSumRows;
-    across = (unsigned)((K + rows - 1 + kBlock - 1) / kBlock);
-    strips = (unsigned)((Q + kSumRows - 1) / kSumRows);
-    down = strips * (unsigned)(own_positions ? B : 1);
-    slots = across * down;
+// Enough wavefronts to fill the GPU, if that can be had: fewer rows for each first, then fewer batches, then fewer rows again.
+constexpr uint64_t kEnough = 4096;
+
+Cut cut_for(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
+  Cut c;
+  c.rows = kMostRows;
+  while (c.rows / 2 >= Q && c.rows > kGroup) c.rows /= 2;
+  c.batches = own_positions ? 1 : (unsigned)B;
+  c.across = (unsigned)((K + kCols - 1) / kCols);
+  for (;;) {
+    c.strips = (unsigned)((Q + c.rows - 1) / c.rows);
+    c.chunks = (unsigned)((B + c.batches - 1) / c.batches);
+    if (c.tiles() * H >= kEnough) break;
+    if (c.rows > 32)
+      c.rows /= 2;
+    else if (c.batches > 1)
+      c.batches = (c.batches + 1) / 2;
+    else if (c.rows > kGroup)
+      c.rows /= 2;
+    else
+      break;
   }
-};
+  return c;
+}
+
+uint64_t groups_of(const Cut& c) { return (c.tiles() + kWaves - 1) / kWaves; }
 
 }  // namespace
 }  // namespace pskv
@@ -232,13 +442,12 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
   }
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
-  const dim3 grid((unsigned)((K + kCols - 1) / kCols), (unsigned)((Q + kRows - 1) / kRows),
-                  (unsigned)(B * H < 65535 ? B * H : 65535));
+  const Cut cut = cut_for(B, H, Q, K, q_at != nullptr);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     auto kernel = scores ? k_relbias<T, true> : k_relbias<T, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, static_cast<hipStream_t>(stream), table, q_at,
-                       static_cast<const T*>(scores), static_cast<T*>(out), s, b);
+    hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles() * H, kWaves, 1u << 22)), dim3(kBlock), 0,
+                       static_cast<hipStream_t>(stream), table, q_at, static_cast<const T*>(scores), static_cast<T*>(out), cut, s, b);
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
@@ -246,7 +455,7 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
 
 extern "C" size_t pskv_relbias_grad_room(size_t buckets, size_t H, size_t B, size_t Q, size_t K, int own_positions) {
   if (B == 0 || Q == 0 || K == 0 || B > (1u << 20) || Q > (1u << 20) || K > (1u << 30)) return 0;
-  return SumPlan(B, Q, K, own_positions != 0).slots * buckets * H * sizeof(float);
+  return groups_of(cut_for(B, H, Q, K, own_positions != 0)) * buckets * H * sizeof(float);
 }
 
 extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void* grad, const int64_t* grad_stride,
@@ -260,16 +469,19 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
   if ((rc = buckets_or_error(&b, buckets, max_distance, two_sided))) return rc;
   if (!grad_table) return set_error(PSKV_EINVAL, "null buffer");
   Shape s{B, H, Q, K, k_first - q_first, {0, 0, 0}, {0, 0, 0}};
-  SumPlan plan(B, Q, K, q_at != nullptr);
   const bool any = B && Q && K;
+  Cut cut{};
+  uint64_t groups = 0;
   if (any) {
     if (!grad) return set_error(PSKV_EINVAL, "null buffer");
     if ((rc = check_strides("grad", grad_stride, s, false))) return rc;
     for (int i = 0; i < 3; ++i) s.in[i] = (uint64_t)grad_stride[i];
-    const size_t room = pskv_relbias_grad_room(buckets, H, B, Q, K, q_at != nullptr);
+    cut = cut_for(B, H, Q, K, q_at != nullptr);
+    groups = groups_of(cut);
+    if (groups > (1u << 23)) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
+    const size_t room = groups * buckets * H * sizeof(float);
     if (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3))
       return set_error(PSKV_EINVAL, "this gradient takes %zu bytes of working memory, %zu given", room, work ? work_bytes : (size_t)0);
-    if (plan.down > 65535) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
   }
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
@@ -278,11 +490,11 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
   if (any)
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      hipLaunchKernelGGL(k_relbias_sums<T>, dim3(plan.across, plan.down, (unsigned)H), dim3(kBlock), 0, st,
-                         static_cast<const T*>(grad), q_at, partial, (unsigned)buckets, plan.slots, plan.strips, s, b);
+      hipLaunchKernelGGL(k_relbias_sums<T>, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad),
+                         q_at, partial, (unsigned)buckets, cut, s, b);
     });
   hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(kBlock), 0, st, partial, (unsigned)buckets,
-                     any ? plan.slots : 0u, (uint64_t)H, grad_table);
+                     (unsigned)groups, (uint64_t)H, grad_table);
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
 }
