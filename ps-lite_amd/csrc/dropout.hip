@@ -17,16 +17,31 @@ namespace {
 constexpr unsigned kBlock = 256;
 constexpr unsigned kDrawn = 8;  // columns that one draw serves
 
-template <typename T>
+// n / d for n below 2^32 by a product (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
+struct Divisor {
+  uint32_t d, magic, shift;
+  explicit Divisor(uint32_t by) : d(by), magic(0), shift(0) {
+    unsigned l = 0;
+    while (l < 32 && (1ull << l) < by) ++l;
+    magic = (uint32_t)(((((1ull << l) - by) << 32) / by) + 1);
+    shift = l;
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const {
+    const uint32_t t = __umulhi(magic, n);
+    return shift == 0 ? n : (t + ((n - t) >> 1)) >> (shift - 1);
+  }
+};
+
+template <typename T, bool FEW>
 __global__ __launch_bounds__(kBlock) void k_dropout(const T* x, T* out, const uint64_t* __restrict__ keys, uint64_t first,
                                                      const uint64_t* __restrict__ step, uint64_t seed, uint64_t n, uint64_t k,
-                                                     uint64_t x_stride, uint64_t out_stride, unsigned least, float scale) {
+                                                     uint64_t x_stride, uint64_t out_stride, unsigned least, float scale, Divisor per_row) {
   using Vec = typename Row<T>::Vec;
   constexpr unsigned W = Row<T>::kWide;
   if (step) seed += *step;
   const uint64_t blocks = (k + kDrawn - 1) / kDrawn;
   for (uint64_t at = (uint64_t)blockIdx.x * kBlock + threadIdx.x; at < n * blocks; at += (uint64_t)gridDim.x * kBlock) {
-    const uint64_t r = at / blocks, q = at % blocks;
+    const uint64_t r = FEW ? per_row.of((uint32_t)at) : at / blocks, q = at - r * blocks;
     const uint64_t key = keys ? keys[r] : first + r;
     const Drawn d = philox((uint32_t)key, (uint32_t)(key >> 32), (uint32_t)q, 0, (uint32_t)seed, (uint32_t)(seed >> 32));
     const T* from = x + r * x_stride + q * kDrawn;
@@ -37,16 +52,16 @@ __global__ __launch_bounds__(kBlock) void k_dropout(const T* x, T* out, const ui
       return bits >= least ? (T)((float)v * scale) : (T)0.0f;
     };
     if (wide == kDrawn) {
-  #pragma unroll
+#pragma unroll
       for (unsigned i = 0; i < kDrawn; i += W) {
         const Vec v = *reinterpret_cast<const Vec*>(from + i);
         Vec o;
-  #pragma unroll
+#pragma unroll
         for (unsigned e = 0; e < W; ++e) o[e] = kept(i + e, v[e]);
         *reinterpret_cast<Vec*>(to + i) = o;
       }
     } else {
-  #pragma unroll
+#pragma unroll
       for (unsigned i = 0; i < kDrawn; ++i)
         if (i < wide) to[i] = kept(i, from[i]);
     }
@@ -82,9 +97,10 @@ extern "C" int pskv_dropout(int device, void* stream, int type, const void* x, s
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL(k_dropout<T>, dim3(grid_for(n * blocks, kBlock, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream),
+    auto kernel = n * blocks < (1ull << 32) ? k_dropout<T, true> : k_dropout<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid_for(n * blocks, kBlock, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream),
                        static_cast<const T*>(x), static_cast<T*>(out), keys, first, step, seed, (uint64_t)n, (uint64_t)k,
-                       (uint64_t)x_stride, (uint64_t)out_stride, least, scale);
+                       (uint64_t)x_stride, (uint64_t)out_stride, least, scale, Divisor((uint32_t)blocks));
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
