@@ -318,7 +318,7 @@ int pskv_match(int device, const uint64_t* src_keys, size_t n_src, const float* 
  *   place[n]      where choice i went, -1 when it is not here
  *   order[n]      the choice that went to p (its token is order[p] / choices), -1 from offsets[E] on
  * `work`: pskv_route_room(n, E) bytes, aligned to 4; none (NULL) where that is 0. */
-#define PSKV_ROUTE_MAX_EXPERTS 4096
+#define PSKV_ROUTE_MAX_EXPERTS 2048
 size_t pskv_route_room(size_t n, size_t E);
 int pskv_route_sort(int device, void* stream, const void* experts, int index_bits, size_t n, size_t E, int32_t* order,
                     int32_t* place, int32_t* offsets, void* work, size_t work_bytes);

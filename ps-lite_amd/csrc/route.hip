@@ -18,10 +18,10 @@ namespace {
 
 constexpr unsigned kSortBlock = 1024;
 constexpr unsigned kSortWaves = kSortBlock / 64;
-constexpr unsigned kSortItems = 8;  // choices per lane
+constexpr unsigned kSortItems = 4;  // choices per lane; one where there are not more of them than lanes
 constexpr unsigned kSortTile = kSortBlock * kSortItems;
 // Up to so many tiles, every workgroup adds up the tiles' counts for itself; beyond, a launch of its own does.
-constexpr unsigned kSortFew = 32;
+constexpr unsigned kSortFew = 128;
 constexpr unsigned kSortBins = PSKV_ROUTE_MAX_EXPERTS + 1;  // the last one in use: choices that are not here
 
 template <typename I>
@@ -36,13 +36,15 @@ __global__ __launch_bounds__(kSortBlock) void k_route_count(const I* __restrict_
                                                              unsigned* __restrict__ counts) {
   __shared__ unsigned hist[kSortBins];
   for (unsigned e = threadIdx.x; e <= E; e += kSortBlock) hist[e] = 0;
-  __syncthreads();
-  const uint64_t first = (uint64_t)blockIdx.x * kSortTile;
+  const uint64_t first = (uint64_t)blockIdx.x * kSortTile + threadIdx.x;
+  unsigned bin[kSortItems];
 #pragma unroll
-  for (unsigned s = 0; s < kSortItems; ++s) {
-    const uint64_t i = first + s * kSortBlock + threadIdx.x;
-    if (i < n) atomicAdd(&hist[bin_of(experts, i, E)], 1u);
-  }
+  for (unsigned s = 0; s < kSortItems; ++s)
+    bin[s] = first + s * kSortBlock < n ? bin_of(experts, first + s * kSortBlock, E) : kSortBins;
+  __syncthreads();
+#pragma unroll
+  for (unsigned s = 0; s < kSortItems; ++s)
+    if (bin[s] < kSortBins) atomicAdd(&hist[bin[s]], 1u);
   __syncthreads();
   for (unsigned e = threadIdx.x; e <= E; e += kSortBlock) counts[(uint64_t)blockIdx.x * (E + 1) + e] = hist[e];
 }
@@ -67,27 +69,47 @@ __global__ __launch_bounds__(64) void k_route_scan(unsigned* __restrict__ counts
   counts[(uint64_t)tiles * bins + e] = run;
 }
 
-// Places of a tile's choices. A wavefront owns 512 neighbouring ones and takes them 64 at a time: lanes of the same bin find
-// each other by comparing the bits of their bins, so a choice's rank among its wavefront's is known without atomics; ranks
-// begin where the earlier wavefronts', tiles' and bins' choices end.
-template <typename I>
+// Places of a tile's choices. A wavefront owns neighbouring ones and takes them 64 at a time: lanes of the same bin find each
+// other by comparing the bits of their bins, so a choice's rank among its wavefront's is known without atomics; ranks begin
+// where the earlier wavefronts', tiles' and bins' choices end.
+template <typename I, unsigned ITEMS>
 __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict__ experts, uint64_t n, unsigned E,
                                                              const unsigned* __restrict__ counts, unsigned tiles,
-                                                             bool scanned, int* __restrict__ order, int* __restrict__ place,
-                                                             int* __restrict__ offsets) {
+                                                             bool scanned, int* __restrict__ order,
+                                                             int* __restrict__ place, int* __restrict__ offsets) {
   __shared__ unsigned short mine[kSortWaves][kSortBins];  // of a wavefront, then of those before it
-  __shared__ unsigned base[kSortBins];
+  __shared__ unsigned total[kSortBins], base[kSortBins];  // of a bin in all tiles, in the tiles before
   __shared__ unsigned sums[kSortWaves];
   const unsigned bins = E + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (unsigned e = lane; e < bins; e += 64) mine[wave][e] = 0;
-  const uint64_t first = (uint64_t)blockIdx.x * kSortTile + wave * (64 * kSortItems) + lane;
-  unsigned bin[kSortItems], rank[kSortItems];
+  const uint64_t first = (uint64_t)blockIdx.x * (kSortBlock * ITEMS) + wave * (64 * ITEMS) + lane;
+  unsigned bin[ITEMS], rank[ITEMS];
 #pragma unroll
-  for (unsigned s = 0; s < kSortItems; ++s) bin[s] = first + s * 64 < n ? bin_of(experts, first + s * 64, E) : bins;
+  for (unsigned s = 0; s < ITEMS; ++s) bin[s] = first + s * 64 < n ? bin_of(experts, first + s * 64, E) : bins;
+  for (unsigned e = lane; e < bins; e += 64) mine[wave][e] = 0;
+  for (unsigned e = threadIdx.x; e < bins; e += kSortBlock) {
+    total[e] = tiles > 1 && scanned ? counts[(uint64_t)tiles * bins + e] : 0;
+    base[e] = tiles > 1 && scanned ? counts[(uint64_t)blockIdx.x * bins + e] : 0;
+  }
+  __syncthreads();
+  if (tiles > 1 && !scanned) {
+    // the counts lie tile by tile: a thread's steps through them are 1,024 apart
+    const unsigned all = tiles * bins, before = blockIdx.x * bins, hop = kSortBlock % bins;
+    unsigned e = threadIdx.x % bins;
+#pragma unroll 8
+    for (unsigned i = threadIdx.x; i < all; i += kSortBlock) {
+      const unsigned c = counts[i];
+      if (c) {
+        atomicAdd(&total[e], c);
+        if (i < before) atomicAdd(&base[e], c);
+      }
+      e += hop;
+      if (e >= bins) e -= bins;
+    }
+  }
   const unsigned bits = 32 - __builtin_clz(bins);
   const uint64_t before = (1ull << lane) - 1;
 #pragma unroll
-  for (unsigned s = 0; s < kSortItems; ++s) {
+  for (unsigned s = 0; s < ITEMS; ++s) {
     uint64_t same = ~0ull;
     for (unsigned b = 0; b < bits; ++b) {
       const bool one = (bin[s] >> b) & 1;
@@ -103,34 +125,25 @@ __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict_
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   __syncthreads();
-  // where every bin begins: its own total over all tiles, summed up over the bins, four to a thread
+  // where every bin begins: the totals summed up over the bins, some to a thread
   constexpr unsigned kPer = (kSortBins + kSortBlock - 1) / kSortBlock;
-  unsigned total[kPer], earlier[kPer], all = 0;
+  const unsigned per = (bins + kSortBlock - 1) / kSortBlock;
+  unsigned amount[kPer], all = 0;
 #pragma unroll
   for (unsigned q = 0; q < kPer; ++q) {
-    const unsigned e = threadIdx.x * kPer + q;
-    total[q] = earlier[q] = 0;
-    if (e < bins) {
+    const unsigned e = threadIdx.x * per + q;
+    amount[q] = 0;
+    if (q < per && e < bins) {
       unsigned run = 0;
+#pragma unroll
       for (unsigned w = 0; w < kSortWaves; ++w) {
         const unsigned c = mine[w][e];
         mine[w][e] = (unsigned short)run;
         run += c;
       }
-      total[q] = run;
-      if (scanned) {
-        total[q] = counts[(uint64_t)tiles * bins + e];
-        earlier[q] = counts[(uint64_t)blockIdx.x * bins + e];
-      } else if (tiles > 1) {
-        total[q] = 0;
-        for (unsigned t = 0; t < tiles; ++t) {
-          const unsigned c = counts[(uint64_t)t * bins + e];
-          total[q] += c;
-          earlier[q] += t < blockIdx.x ? c : 0;
-        }
-      }
+      amount[q] = tiles > 1 ? total[e] : run;
     }
-    all += total[q];
+    all += amount[q];
   }
   unsigned inc = all;
 #pragma unroll
@@ -144,16 +157,16 @@ __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict_
   for (unsigned w = 0; w < wave; ++w) run += sums[w];
 #pragma unroll
   for (unsigned q = 0; q < kPer; ++q) {
-    const unsigned e = threadIdx.x * kPer + q;
-    if (e < bins) {
-      base[e] = run + earlier[q];
+    const unsigned e = threadIdx.x * per + q;
+    if (q < per && e < bins) {
+      base[e] += run;
       if (blockIdx.x == 0) offsets[e] = (int)run;
     }
-    run += total[q];
+    run += amount[q];
   }
   __syncthreads();
 #pragma unroll
-  for (unsigned s = 0; s < kSortItems; ++s) {
+  for (unsigned s = 0; s < ITEMS; ++s) {
     if (bin[s] >= bins) continue;
     const uint64_t i = first + s * 64;
     const unsigned p = base[bin[s]] + mine[wave][bin[s]] + rank[s];
@@ -173,14 +186,22 @@ struct RowArgs {
   unsigned choices, lanes_log2;
 };
 
-template <typename T>
+// The token of a lane; where a wavefront or more serves one, the compiler is told that all lanes have the same, so that places and
+// weights are loaded once per wavefront.
+template <bool ONE>
+__device__ __forceinline__ uint64_t token_of(uint64_t t) {
+  if (!ONE) return t;
+  return (uint64_t)__builtin_amdgcn_readfirstlane((int)(t >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)t);
+}
+
+template <typename T, bool ONE>
 __global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ x, const int* __restrict__ place,
                                                            T* __restrict__ out, RowArgs a) {
   using Vec = typename Row<T>::Vec;
   constexpr unsigned W = Row<T>::kWide;
   const unsigned lanes = 1u << a.lanes_log2;
   const uint64_t per = (uint64_t)gridDim.x * (kRowBlock >> a.lanes_log2);
-  for (uint64_t t = ((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2; t < a.tokens; t += per) {
+  for (uint64_t t = token_of<ONE>(((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2); t < a.tokens; t += per) {
     const T* from = x + t * a.token_stride;
     const int* at = place + t * a.choices;
     for (uint64_t c = (uint64_t)(threadIdx.x & (lanes - 1)) * W; c < a.k; c += (uint64_t)lanes * W) {
@@ -201,42 +222,58 @@ __global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ 
   }
 }
 
-template <typename T>
+// Eight answers are asked for at a time. A choice that is not here reads row 0, whose elements are replaced by zeros.
+template <typename T, bool ONE>
 __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ rows, const int* __restrict__ place,
                                                           const float* __restrict__ weights, T* __restrict__ out, RowArgs a) {
   using Vec = typename Row<T>::Vec;
-  constexpr unsigned W = Row<T>::kWide;
+  constexpr unsigned W = Row<T>::kWide, kAhead = 8;
   const unsigned lanes = 1u << a.lanes_log2;
   const uint64_t per = (uint64_t)gridDim.x * (kRowBlock >> a.lanes_log2);
-  for (uint64_t t = ((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2; t < a.tokens; t += per) {
+  for (uint64_t t = token_of<ONE>(((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2); t < a.tokens; t += per) {
     const int* at = place + t * a.choices;
     const float* w = weights ? weights + t * a.choices : nullptr;
     T* to = out + t * a.token_stride;
     for (uint64_t c = (uint64_t)(threadIdx.x & (lanes - 1)) * W; c < a.k; c += (uint64_t)lanes * W) {
-      const unsigned wide = c + W <= a.k ? W : (unsigned)(a.k - c);
       float sum[W] = {};
-      for (unsigned j = 0; j < a.choices; ++j) {
-        const uint64_t p = (uint64_t)(int64_t)at[j];
-        if (p >= a.rows) continue;
-        const float f = w ? w[j] : 1.0f;
-        const T* from = rows + p * a.row_stride + c;
-        if (wide == W) {
-          const Vec v = *reinterpret_cast<const Vec*>(from);
-  #pragma unroll
-          for (unsigned i = 0; i < W; ++i) sum[i] = __builtin_fmaf(f, (float)v[i], sum[i]);
-        } else {
-  #pragma unroll
-          for (unsigned i = 0; i < W; ++i)
-            if (i < wide) sum[i] = __builtin_fmaf(f, (float)from[i], sum[i]);
-        }
-      }
-      if (wide == W) {
+      if (c + W <= a.k) {
+        auto some = [&](unsigned j0, auto count) {
+          constexpr unsigned N = decltype(count)::value;
+          Vec v[N];
+          bool here[N];
+#pragma unroll
+          for (unsigned j = 0; j < N; ++j) {
+            const uint64_t p = (uint64_t)(int64_t)at[j0 + j];
+            here[j] = p < a.rows;
+            v[j] = *reinterpret_cast<const Vec*>(rows + (here[j] ? p : 0) * a.row_stride + c);
+          }
+#pragma unroll
+          for (unsigned j = 0; j < N; ++j) {
+            const float f = !here[j] ? 0.0f : w ? w[j0 + j] : 1.0f;
+#pragma unroll
+            for (unsigned i = 0; i < W; ++i) sum[i] = __builtin_fmaf(f, here[j] ? (float)v[j][i] : 0.0f, sum[i]);
+          }
+        };
+        unsigned j = 0;
+        for (; j + kAhead <= a.choices; j += kAhead) some(j, std::integral_constant<unsigned, kAhead>());
+        if (a.choices & 4) some(j, std::integral_constant<unsigned, 4>()), j += 4;
+        if (a.choices & 2) some(j, std::integral_constant<unsigned, 2>()), j += 2;
+        if (a.choices & 1) some(j, std::integral_constant<unsigned, 1>());
         Vec v;
-  #pragma unroll
+#pragma unroll
         for (unsigned i = 0; i < W; ++i) v[i] = (T)sum[i];
         *reinterpret_cast<Vec*>(to + c) = v;
       } else {
-  #pragma unroll
+        const unsigned wide = (unsigned)(a.k - c);
+        for (unsigned j = 0; j < a.choices; ++j) {
+          const uint64_t p = (uint64_t)(int64_t)at[j];
+          if (p >= a.rows) continue;
+          const float f = w ? w[j] : 1.0f;
+#pragma unroll
+          for (unsigned i = 0; i < W; ++i)
+            if (i < wide) sum[i] = __builtin_fmaf(f, (float)rows[p * a.row_stride + c + i], sum[i]);
+        }
+#pragma unroll
         for (unsigned i = 0; i < W; ++i)
           if (i < wide) to[c + i] = (T)sum[i];
       }
@@ -244,8 +281,11 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ r
   }
 }
 
-// At most a wavefront per token, so that the products' sums need no other than its own lanes.
-template <typename T>
+// At most a wavefront per token, so that the products' sums need no other than its own lanes. A lane keeps its part of the
+// token's gradient, up to kKept vectors of it, for all choices, and asks for the next answer before it uses one.
+constexpr unsigned kKept = 4;
+
+template <typename T, bool ONE>
 __global__ __launch_bounds__(kRowBlock) void k_route_sum_grad(const T* __restrict__ grad, const T* __restrict__ rows,
                                                                const int* __restrict__ place,
                                                                const float* __restrict__ weights, T* __restrict__ grad_rows,
@@ -253,35 +293,53 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum_grad(const T* __restric
                                                                RowArgs a) {
   using Vec = typename Row<T>::Vec;
   constexpr unsigned W = Row<T>::kWide;
-  const unsigned lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1), own = threadIdx.x >> a.lanes_log2;
+  const unsigned lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const uint64_t per = kRowBlock >> a.lanes_log2;
+  const uint64_t wide = (uint64_t)lanes * W, whole = a.k / W * W;  // elements of a vector for all lanes; of whole vectors
   for (uint64_t t0 = blockIdx.x * per; t0 < a.tokens; t0 += gridDim.x * per) {
-    const uint64_t t = t0 + own;
+    const uint64_t t = token_of<ONE>(t0 + (threadIdx.x >> a.lanes_log2));
     const bool is = t < a.tokens;  // (no lane leaves: they add up together)
-    const T* g = grad + t * a.token_stride;
+    const T* g = grad + (is ? t : 0) * a.token_stride;
+    const int* at = place + (is ? t : 0) * a.choices;
+    const float* w = weights + (is ? t : 0) * a.choices;
+    Vec d[kKept], v[kKept];
+    const bool kept = whole <= kKept * wide;
+    if (kept) {
+#pragma unroll
+      for (unsigned q = 0; q < kKept; ++q)
+        if (lane * W + q * wide < whole) d[q] = *reinterpret_cast<const Vec*>(g + lane * W + q * wide);
+    }
     for (unsigned j = 0; j < a.choices; ++j) {
-      const uint64_t p = is ? (uint64_t)(int64_t)place[t * a.choices + j] : ~0ull;
+      const uint64_t p = is ? (uint64_t)(int64_t)at[j] : ~0ull;
       float sum = 0.0f;
       if (p < a.rows) {
-        const float f = weights[t * a.choices + j];
+        const float f = w[j];
         const T* from = rows + p * a.row_stride;
         T* to = grad_rows + p * grad_row_stride;
-        for (uint64_t c = (uint64_t)lane * W; c < a.k; c += (uint64_t)lanes * W) {
-          if (c + W <= a.k) {
-            const Vec d = *reinterpret_cast<const Vec*>(g + c), v = *reinterpret_cast<const Vec*>(from + c);
-            Vec o;
-  #pragma unroll
-            for (unsigned i = 0; i < W; ++i) {
-              sum = __builtin_fmaf((float)d[i], (float)v[i], sum);
-              o[i] = (T)(f * (float)d[i]);
-            }
-            *reinterpret_cast<Vec*>(to + c) = o;
-          } else {
-            for (uint64_t i = c; i < a.k; ++i) {
-              sum = __builtin_fmaf((float)g[i], (float)from[i], sum);
-              to[i] = (T)(f * (float)g[i]);
-            }
+        for (uint64_t c0 = lane * W; c0 < whole; c0 += kKept * wide) {
+#pragma unroll
+          for (unsigned q = 0; q < kKept; ++q)
+            if (c0 + q * wide < whole) v[q] = *reinterpret_cast<const Vec*>(from + c0 + q * wide);
+          if (!kept) {
+#pragma unroll
+            for (unsigned q = 0; q < kKept; ++q)
+              if (c0 + q * wide < whole) d[q] = *reinterpret_cast<const Vec*>(g + c0 + q * wide);
           }
+#pragma unroll
+          for (unsigned q = 0; q < kKept; ++q)
+            if (c0 + q * wide < whole) {
+              Vec o;
+#pragma unroll
+              for (unsigned i = 0; i < W; ++i) {
+                sum = __builtin_fmaf((float)d[q][i], (float)v[q][i], sum);
+                o[i] = (T)(f * (float)d[q][i]);
+              }
+              *reinterpret_cast<Vec*>(to + c0 + q * wide) = o;
+            }
+        }
+        for (uint64_t i = whole + lane; i < a.k; i += lanes) {
+          sum = __builtin_fmaf((float)g[i], (float)from[i], sum);
+          to[i] = (T)(f * (float)g[i]);
         }
       }
       for (unsigned o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
@@ -357,7 +415,7 @@ extern "C" int pskv_route_sort(int device, void* stream, const void* experts, in
     using I = std::remove_const_t<std::remove_pointer_t<decltype(e)>>;
     if (tiles > 1) hipLaunchKernelGGL(k_route_count<I>, dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts);
     if (scanned) hipLaunchKernelGGL(k_route_scan, dim3((unsigned)E / 64 + 1), dim3(64), 0, st, counts, tiles, (unsigned)E + 1);
-    hipLaunchKernelGGL(k_route_place<I>, dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts, tiles, scanned,
+    hipLaunchKernelGGL((n <= kSortBlock ? k_route_place<I, 1> : k_route_place<I, kSortItems>), dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts, tiles, scanned,
                        order, place, offsets);
   };
   if (index_bits == 64)
@@ -384,7 +442,8 @@ extern "C" int pskv_route_rows(int device, void* stream, int type, const void* x
   const RowArgs a = row_args(tokens, choices, n_rows, k, x_stride, rows_stride, type, kRowBlock);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL(k_route_rows<T>, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+    auto kernel = a.lanes_log2 >= 6 ? k_route_rows<T, true> : k_route_rows<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
                        static_cast<hipStream_t>(stream), static_cast<const T*>(x), place, static_cast<T*>(rows), a);
   });
   PSKV_HIP(hipGetLastError());
@@ -405,10 +464,12 @@ extern "C" int pskv_route_sum(int device, void* stream, int type, const void* ro
     return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
-  const RowArgs a = row_args(tokens, choices, n_rows, k, out_stride, rows_stride, type, kRowBlock);
+  // (without rows there is no row 0 to read either)
+  const RowArgs a = row_args(tokens, n_rows ? choices : 0, n_rows, k, out_stride, rows_stride, type, kRowBlock);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL(k_route_sum<T>, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+    auto kernel = a.lanes_log2 >= 6 ? k_route_sum<T, true> : k_route_sum<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
                        static_cast<hipStream_t>(stream), static_cast<const T*>(rows), place, weights, static_cast<T*>(out), a);
   });
   PSKV_HIP(hipGetLastError());
@@ -436,7 +497,8 @@ extern "C" int pskv_route_sum_grad(int device, void* stream, int type, const voi
   const RowArgs a = row_args(tokens, choices, n_rows, k, grad_stride, rows_stride, type, 64);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    hipLaunchKernelGGL(k_route_sum_grad<T>, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+    auto kernel = a.lanes_log2 >= 6 ? k_route_sum_grad<T, true> : k_route_sum_grad<T, false>;
+    hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
                        static_cast<hipStream_t>(stream), static_cast<const T*>(grad), static_cast<const T*>(rows), place, weights,
                        static_cast<T*>(grad_rows), (uint64_t)grad_rows_stride, grad_weights, a);
   });

@@ -14,7 +14,7 @@ or ValueError, what the library refuses raises PskvError.
 from . import capi
 from .capi import _check
 
-MAX_EXPERTS = 4096
+MAX_EXPERTS = 2048
 MAX_BUCKETS = 256
 
 

@@ -79,9 +79,9 @@ def sort(ops, experts, E, **more):
 
 
 @pytest.mark.parametrize("bits", [32, 64])
-@pytest.mark.parametrize("T,K,E", [(0, 2, 5), (1, 1, 1), (1, 2, 4096), (7, 3, 2), (64, 1, 7), (65, 8, 63), (1000, 3, 64), (513, 5, 65),
-                                   (1024, 8, 256), (8193, 1, 8), (4099, 6, 1000), (2731, 3, 4096), (100003, 3, 60),
-                                   (262145, 1, 1), (300007, 1, 4095)])
+@pytest.mark.parametrize("T,K,E", [(0, 2, 5), (1, 1, 1), (1, 2, 2048), (7, 3, 2), (64, 1, 7), (65, 8, 63), (1000, 3, 64), (513, 5, 65),
+                                   (1024, 8, 256), (8193, 1, 8), (1025, 1, 8), (4096, 1, 9), (4097, 1, 300), (4099, 6, 1000), (2731, 3, 2048), (100003, 3, 60),
+                                   (262145, 1, 1), (600007, 1, 2047)])
 @pytest.mark.parametrize("lost", [0.0, 0.3, 1.0])
 def test_sort(ops, dev, bits, T, K, E, lost):
     import torch
