@@ -17,6 +17,11 @@ namespace {
 constexpr unsigned kBlock = 256;
 constexpr unsigned kDrawn = 8;  // columns that one draw serves
 
+template <typename T>
+__device__ __forceinline__ T keep(uint32_t word, bool high, unsigned least, T v, float scale) {
+  return (high ? word >> 16 : word & 0xffffu) >= least ? (T)((float)v * scale) : (T)0.0f;
+}
+
 // n / d for n below 2^32 by a product (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994).
 struct Divisor {
   uint32_t d, magic, shift;
@@ -32,7 +37,7 @@ struct Divisor {
   }
 };
 
-template <typename T, bool FEW>
+template <typename T, bool FEW, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_dropout(const T* x, T* out, const uint64_t* __restrict__ keys, uint64_t first,
                                                      const uint64_t* __restrict__ step, uint64_t seed, uint64_t n, uint64_t k,
                                                      uint64_t x_stride, uint64_t out_stride, unsigned least, float scale, Divisor per_row) {
@@ -43,28 +48,77 @@ __global__ __launch_bounds__(kBlock) void k_dropout(const T* x, T* out, const ui
   for (uint64_t at = (uint64_t)blockIdx.x * kBlock + threadIdx.x; at < n * blocks; at += (uint64_t)gridDim.x * kBlock) {
     const uint64_t r = FEW ? per_row.of((uint32_t)at) : at / blocks, q = at - r * blocks;
     const uint64_t key = keys ? keys[r] : first + r;
+    const uint64_t c = q * kDrawn;
     const Drawn d = philox((uint32_t)key, (uint32_t)(key >> 32), (uint32_t)q, 0, (uint32_t)seed, (uint32_t)(seed >> 32));
-    const T* from = x + r * x_stride + q * kDrawn;
-    T* to = out + r * out_stride + q * kDrawn;
-    const unsigned wide = k - q * kDrawn < kDrawn ? (unsigned)(k - q * kDrawn) : kDrawn;
-    auto kept = [&](unsigned i, T v) {
-      const unsigned bits = i & 1 ? d.word[i / 2] >> 16 : d.word[i / 2] & 0xffffu;
-      return bits >= least ? (T)((float)v * scale) : (T)0.0f;
-    };
-    if (wide == kDrawn) {
+    const T* from = x + r * x_stride + c;
+    T* to = out + r * out_stride + c;
+    auto kept = [&](unsigned i, T v) { return keep(d.word[i / 2], i & 1, least, v, scale); };
+    if (k - c >= kDrawn) {
 #pragma unroll
       for (unsigned i = 0; i < kDrawn; i += W) {
-        const Vec v = *reinterpret_cast<const Vec*>(from + i);
+        const Vec v = get<PAST>(from + i);
         Vec o;
 #pragma unroll
         for (unsigned e = 0; e < W; ++e) o[e] = kept(i + e, v[e]);
-        *reinterpret_cast<Vec*>(to + i) = o;
+        put<PAST>(to + i, o);
       }
     } else {
 #pragma unroll
       for (unsigned i = 0; i < kDrawn; ++i)
-        if (i < wide) to[i] = kept(i, from[i]);
+        if (i < k - c) to[i] = kept(i, from[i]);
     }
+  }
+}
+
+__device__ __forceinline__ uint32_t of_neighbour(uint32_t v) {  // lanes 2i and 2i + 1 exchange
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1 /* quad_perm:[1,0,3,2] */, 0xf, 0xf, false);
+}
+
+// float32: a draw's 8 columns are 32 bytes, and lanes that each take 32 bytes leave every access half of its lines. So a lane
+// takes four columns here and four 64 lanes further on; of two neighbours the even one draws for both here, the odd one there,
+// and they exchange halves. Indexes are those of quads of columns, two to a draw.
+template <bool PAST>
+__global__ __launch_bounds__(kBlock) void k_dropout_pairs(const float* x, float* out, const uint64_t* __restrict__ keys, uint64_t first,
+                                                           const uint64_t* __restrict__ step, uint64_t seed, uint32_t quads, uint32_t k,
+                                                           uint64_t x_stride, uint64_t out_stride, unsigned least, float scale,
+                                                           Divisor per_row) {
+  using Vec = Row<float>::Vec;
+  if (step) seed += *step;
+  const unsigned lane = threadIdx.x & 63;
+  const bool odd = lane & 1;
+  const uint32_t here = (blockIdx.x * kBlock + threadIdx.x - lane) * 2 + lane;
+  const uint32_t mine = odd ? here + 64 : here;
+  const uint32_t r = per_row.of(mine), q = mine - r * per_row.d;
+  uint64_t key = first + r;
+  if (keys && mine < quads) key = keys[r];
+  const Drawn d = philox((uint32_t)key, (uint32_t)(key >> 32), q >> 1, 0, (uint32_t)seed, (uint32_t)(seed >> 32));
+  const uint32_t other0 = of_neighbour(odd ? d.word[0] : d.word[2]), other1 = of_neighbour(odd ? d.word[1] : d.word[3]);
+  const uint32_t other_r = of_neighbour(r), other_q = of_neighbour(q);
+  // (the lower half of the draw is the even lane's)
+  const uint32_t rows[2] = {odd ? other_r : r, odd ? r : other_r};
+  const uint32_t cols[2] = {(((odd ? other_q : q) & ~1u) + (odd ? 1 : 0)) * 4, (((odd ? q : other_q) & ~1u) + (odd ? 1 : 0)) * 4};
+  const uint32_t words[2][2] = {{odd ? other0 : d.word[0], odd ? other1 : d.word[1]}, {odd ? d.word[2] : other0, odd ? d.word[3] : other1}};
+  Vec v[2];
+  bool whole[2];
+#pragma unroll
+  for (unsigned h = 0; h < 2; ++h) {
+    const bool is = here + h * 64 < quads && cols[h] < k;
+    whole[h] = is && k - cols[h] >= 4;
+    const float* from = x + rows[h] * x_stride + cols[h];
+    if (whole[h]) v[h] = get<PAST>(from);
+    if (is && !whole[h]) {
+      float* to = out + rows[h] * out_stride + cols[h];
+#pragma unroll
+      for (unsigned i = 0; i < 3; ++i)
+        if (i < k - cols[h]) to[i] = keep(words[h][i / 2], i & 1, least, from[i], scale);
+    }
+  }
+#pragma unroll
+  for (unsigned h = 0; h < 2; ++h) {
+    Vec o;
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) o[i] = keep(words[h][i / 2], i & 1, least, v[h][i], scale);
+    if (whole[h]) put<PAST>(out + rows[h] * out_stride + cols[h], o);
   }
 }
 
@@ -95,12 +149,22 @@ extern "C" int pskv_dropout(int device, void* stream, int type, const void* x, s
   const float scale = least < 65536 ? (float)(65536.0 / (65536 - least)) : 0.0f;
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
-  with_type(type, [&](auto* t) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    auto kernel = n * blocks < (1ull << 32) ? k_dropout<T, true> : k_dropout<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(grid_for(n * blocks, kBlock, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const T*>(x), static_cast<T*>(out), keys, first, step, seed, (uint64_t)n, (uint64_t)k,
-                       (uint64_t)x_stride, (uint64_t)out_stride, least, scale, Divisor((uint32_t)blocks));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  with_flag(2 * n * k * size > kPastBytes, [&](auto far) {
+    constexpr bool PAST = decltype(far)::value;
+    if (type == PSKV_F32 && n * blocks < (1ull << 31) - kBlock) {
+      hipLaunchKernelGGL(k_dropout_pairs<PAST>, dim3((unsigned)((n * blocks + kBlock - 1) / kBlock)), dim3(kBlock), 0, st,
+                         static_cast<const float*>(x), static_cast<float*>(out), keys, first, step, seed, (uint32_t)(2 * n * blocks),
+                         (uint32_t)k, (uint64_t)x_stride, (uint64_t)out_stride, least, scale, Divisor((uint32_t)(2 * blocks)));
+      return;
+    }
+    with_type(type, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      auto kernel = n * blocks < (1ull << 32) ? k_dropout<T, true, PAST> : k_dropout<T, false, PAST>;
+      hipLaunchKernelGGL(kernel, dim3(grid_for(n * blocks, kBlock, 1u << 22)), dim3(kBlock), 0, st, static_cast<const T*>(x),
+                         static_cast<T*>(out), keys, first, step, seed, (uint64_t)n, (uint64_t)k, (uint64_t)x_stride,
+                         (uint64_t)out_stride, least, scale, Divisor((uint32_t)blocks));
+    });
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;

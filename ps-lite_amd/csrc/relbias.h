@@ -29,18 +29,22 @@ struct Buckets {
   unsigned exact;
   unsigned steps;   // borders in use
   unsigned two_sided;
+  float log_exact, per_log;  // log2(exact), buckets per doubling of the distance
   uint32_t border[kMostBuckets / 2];
 };
 
-// The row of a relative position. The borders are compared one by one: they are the same for all lanes, so they lie in scalar
-// registers, and near positions need none.
-PSKV_BOTH inline unsigned bucket_of(const Buckets& b, int64_t rel) {
+// The row of a relative position. The logarithm in float tells where to look (it is off by one at most), the borders decide;
+// near positions need neither. `border` is b.border, where it can be read fastest.
+PSKV_BOTH inline unsigned bucket_of(const Buckets& b, const uint32_t* border, int64_t rel) {
   const uint64_t far = b.two_sided && rel > 0 ? (uint64_t)rel : rel < 0 ? 0 - (uint64_t)rel : 0;
   const uint32_t d = far > kMostDistance ? (uint32_t)kMostDistance : (uint32_t)far;
   unsigned row = d;
   if (d >= b.exact) {
-    row = b.exact;
-    for (unsigned c = 0; c < b.steps; ++c) row += d >= b.border[c] ? 1 : 0;
+    const float guess = (log2f((float)d) - b.log_exact) * b.per_log;
+    unsigned c = guess <= 0.0f ? 0 : guess >= (float)b.steps ? b.steps : (unsigned)guess;
+    while (c < b.steps && d >= border[c]) ++c;
+    while (c > 0 && d < border[c - 1]) --c;
+    row = b.exact + c;
   }
   return b.two_sided && rel > 0 ? b.side + row : row;
 }
@@ -93,6 +97,8 @@ inline bool make_buckets(Buckets* b, uint64_t buckets, uint64_t max_distance, bo
   if (max_distance <= b->exact) return false;
   const unsigned n = b->side - b->exact;
   b->steps = n - 1;
+  b->log_exact = (float)log2((double)b->exact);
+  b->per_log = (float)(n / log2((double)max_distance / b->exact));
   const double grow = log((double)max_distance / b->exact) / n;
   for (unsigned c = 1; c < n; ++c) {
     const double r = b->exact * exp(grow * c);

@@ -20,6 +20,7 @@ constexpr unsigned kWide = 8;            // neighbouring columns of a lane
 constexpr unsigned kCols = 64 * kWide;   // of a wavefront
 constexpr unsigned kGroup = 8;           // rows that a wavefront asks for before it uses them
 constexpr unsigned kMostRows = 128;      // of a wavefront
+constexpr uint64_t kMostTiles = 1u << 31;
 
 struct Shape {
   uint64_t B, H, Q, K;
@@ -27,11 +28,11 @@ struct Shape {
   uint64_t in[3], out[3];  // strides of batch, head and row
 };
 
-// How a call is cut up: a wavefront takes `rows` rows of kCols columns of one head, for `batches` batches one after the other.
+// How a call is cut up: a wavefront takes `rows` rows of kCols columns, for `heads` heads and `batches` batches one after the other.
 struct Cut {
-  unsigned rows, batches;
-  unsigned across, strips, chunks;  // how many there are of columns, rows, batches
-  __host__ __device__ uint64_t tiles() const { return (uint64_t)across * strips * chunks; }  // of a head
+  unsigned rows, heads, batches;
+  unsigned across, strips, parts, chunks;  // how many there are of columns, rows, heads, batches
+  uint64_t tiles() const { return (uint64_t)across * strips * parts * chunks; }
 };
 
 // Eight neighbouring elements, as they are in memory and as numbers.
@@ -139,71 +140,91 @@ struct Span {
 
 // The tile of a wavefront.
 struct Tile {
-  uint64_t c0, r0, head, batch0;
-  unsigned rows, batches;
-  __device__ __forceinline__ Tile(uint64_t tile, const Cut& cut, uint64_t B, uint64_t H, uint64_t Q) {
-    c0 = tile % cut.across * kCols;
+  uint64_t c0, r0;
+  unsigned head0, batch0, rows, heads, batches;
+  __device__ __forceinline__ Tile(unsigned tile, const Cut& cut, const Shape& s) {
+    c0 = (uint64_t)(tile % cut.across) * kCols;
     tile /= cut.across;
-    r0 = tile % cut.strips * cut.rows;
+    r0 = (uint64_t)(tile % cut.strips) * cut.rows;
     tile /= cut.strips;
-    head = tile % H;
-    batch0 = tile / H * cut.batches;
-    rows = Q - r0 < cut.rows ? (unsigned)(Q - r0) : cut.rows;
-    batches = B - batch0 < cut.batches ? (unsigned)(B - batch0) : cut.batches;
+    head0 = tile % cut.parts * cut.heads;
+    batch0 = tile / cut.parts * cut.batches;
+    rows = s.Q - r0 < cut.rows ? (unsigned)(s.Q - r0) : cut.rows;
+    heads = (unsigned)s.H - head0 < cut.heads ? (unsigned)s.H - head0 : cut.heads;
+    batches = (unsigned)s.B - batch0 < cut.batches ? (unsigned)s.B - batch0 : cut.batches;
   }
 };
+
+// The borders in LDS, for the workgroup. (A barrier has to follow.)
+__device__ __forceinline__ void fetch_borders(uint32_t* to, const Buckets& b) {
+  for (unsigned c = threadIdx.x; c < b.steps; c += kBlock) to[c] = b.border[c];
+}
 
 // A tile of the bias. Row i's bias is row i - 1's, moved one column to the right, so eight rows further down a lane needs what
 // the lane below had: eight values of a lane's own and eight that it is handed serve eight rows, and nothing is looked up
 // but the tile's first row and, for lane 0, its first column, which waits in LDS.
 template <typename T, bool SCORES>
 __global__ __launch_bounds__(kBlock) void k_relbias(const float* __restrict__ table, const int64_t* __restrict__ q_at,
-                                                     const T* scores, T* out, Cut cut, Shape s, Buckets b) {
+                                                     const T* scores, T* out, unsigned tiles, Cut cut, Shape s, Buckets b) {
+  __shared__ uint32_t border[kMostBuckets / 2];
   __shared__ float left[kWaves][kMostRows];  // diagonals -1, -2, ... of the wavefront's tile
-  const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const uint64_t tiles = cut.tiles() * s.H;
-  for (uint64_t tile = (uint64_t)blockIdx.x * kWaves + wave; tile < tiles; tile += (uint64_t)gridDim.x * kWaves) {
-    const Tile t(tile, cut, s.B, s.H, s.Q);
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  fetch_borders(border, b);
+  __syncthreads();
+  for (unsigned tile = blockIdx.x * kWaves + wave; tile < tiles; tile += gridDim.x * kWaves) {
+    const Tile t(tile, cut, s);
     const Span span(t.c0, lane, s.K);
     const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0;
-    auto value = [&](uint64_t r) { return table[(uint64_t)bucket_of(b, (int64_t)r) * s.H + t.head]; };
     const unsigned reach = (t.rows + kGroup - 1) / kGroup * kGroup;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (unsigned i = lane; i < reach; i += 64) left[wave][i] = value(rel - 1 - i);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    float v[kWide], next[kWide];
+    unsigned row[kWide], below[kMostRows / 64];  // of the table, for the tile's first row and its first column
 #pragma unroll
-    for (unsigned k = 0; k < kWide; ++k) v[k] = value(rel + lane * kWide + k);
-    const T* from = SCORES ? scores + t.batch0 * s.in[0] + t.head * s.in[1] + t.r0 * s.in[2] : nullptr;
-    T* to = out + t.batch0 * s.out[0] + t.head * s.out[1] + t.r0 * s.out[2] + t.c0 + lane * kWide;
-    for (unsigned i = 0; i < t.rows; i += kGroup) {
+    for (unsigned k = 0; k < kWide; ++k) row[k] = bucket_of(b, border, (int64_t)(rel + lane * kWide + k)) * (unsigned)s.H;
 #pragma unroll
-      for (unsigned k = 0; k < kWide; ++k) next[k] = from_below(v[k], left[wave][i + kGroup - 1 - k]);
-      auto group = [&](auto whole) {
-        for (unsigned n = 0; n < t.batches; ++n) {
-          Eight<T> x[kGroup];
+    for (unsigned q = 0; q < kMostRows / 64; ++q)
+      below[q] = q * 64 < reach ? bucket_of(b, border, (int64_t)(rel - 1 - q * 64 - lane)) * (unsigned)s.H : 0;
+    const T* from0 = SCORES ? scores + t.batch0 * s.in[0] + t.head0 * s.in[1] + t.r0 * s.in[2] : nullptr;
+    T* to0 = out + t.batch0 * s.out[0] + t.head0 * s.out[1] + t.r0 * s.out[2] + t.c0 + lane * kWide;
+    for (unsigned h = 0; h < t.heads; ++h) {
+      const float* column = table + t.head0 + h;
+      float v[kWide], next[kWide];
 #pragma unroll
-          for (unsigned r = 0; r < kGroup; ++r)
-            if (SCORES && (whole || i + r < t.rows)) span.load(x[r], from + n * s.in[0] + (uint64_t)(i + r) * s.in[2]);
+      for (unsigned k = 0; k < kWide; ++k) v[k] = column[row[k]];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-          for (unsigned r = 0; r < kGroup; ++r) {
-            if (!whole && i + r >= t.rows) continue;
-            float y[kWide];
+      for (unsigned q = 0; q < kMostRows / 64; ++q)
+        if (q * 64 < reach) left[wave][q * 64 + lane] = column[below[q]];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const T* from = SCORES ? from0 + h * s.in[1] : nullptr;
+      T* to = to0 + h * s.out[1];
+      for (unsigned i = 0; i < t.rows; i += kGroup) {
 #pragma unroll
-            for (unsigned k = 0; k < kWide; ++k) {
-              y[k] = k >= r ? v[k - r] : next[kWide + k - r];
-              if (SCORES) y[k] = x[r].at(k) + y[k];
+        for (unsigned k = 0; k < kWide; ++k) next[k] = from_below(v[k], left[wave][i + kGroup - 1 - k]);
+        auto group = [&](auto whole) {
+          for (unsigned n = 0; n < t.batches; ++n) {
+            Eight<T> x[kGroup];
+#pragma unroll
+            for (unsigned r = 0; r < kGroup; ++r)
+              if (SCORES && (whole || i + r < t.rows)) span.load(x[r], from + n * s.in[0] + (uint64_t)(i + r) * s.in[2]);
+#pragma unroll
+            for (unsigned r = 0; r < kGroup; ++r) {
+              if (!whole && i + r >= t.rows) continue;
+              float y[kWide];
+#pragma unroll
+              for (unsigned k = 0; k < kWide; ++k) {
+                y[k] = k >= r ? v[k - r] : next[kWide + k - r];
+                if (SCORES) y[k] = x[r].at(k) + y[k];
+              }
+              store_eight(to + n * s.out[0] + (uint64_t)(i + r) * s.out[2], y, span.own);
             }
-            store_eight(to + n * s.out[0] + (uint64_t)(i + r) * s.out[2], y, span.own);
           }
-        }
-      };
-      if (i + kGroup <= t.rows)
-        group(std::true_type());
-      else
-        group(std::false_type());
+        };
+        if (i + kGroup <= t.rows)
+          group(std::true_type());
+        else
+          group(std::false_type());
 #pragma unroll
-      for (unsigned k = 0; k < kWide; ++k) v[k] = next[k];
+        for (unsigned k = 0; k < kWide; ++k) v[k] = next[k];
+      }
     }
   }
 }
@@ -215,16 +236,19 @@ __global__ __launch_bounds__(kBlock) void k_relbias(const float* __restrict__ ta
 // at a time. Every sum has one order. partial[head][bucket][workgroup of the head].
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ grad, const int64_t* __restrict__ q_at,
-                                                          float* __restrict__ partial, unsigned buckets, Cut cut, Shape s,
-                                                          Buckets b) {
+                                                          float* __restrict__ partial, unsigned buckets, unsigned tiles,
+                                                          Cut cut, Shape s, Buckets b) {
+  __shared__ uint32_t border[kMostBuckets / 2];
   __shared__ float diagonal[kWaves][kMostRows + kCols];
   __shared__ float sums[kWaves][kMostBuckets];
-  const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const uint64_t head = blockIdx.y, tile = (uint64_t)blockIdx.x * kWaves + wave;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint64_t head = blockIdx.y;
+  const unsigned tile = blockIdx.x * kWaves + wave;
+  fetch_borders(border, b);
   for (unsigned u = lane; u < buckets; u += 64) sums[wave][u] = 0.0f;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  if (tile < cut.tiles()) {
-    const Tile t(tile, cut, s.B, 1, s.Q);  // (of this head)
+  __syncthreads();
+  if (tile < tiles) {
+    const Tile t(tile, cut, s);  // (of any head: cut.parts is 1)
     const Span span(t.c0, lane, s.K);
     const T* from = grad + t.batch0 * s.in[0] + head * s.in[1] + t.r0 * s.in[2];
     const unsigned reach = (t.rows + kGroup - 1) / kGroup * kGroup;
@@ -269,19 +293,36 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // diagonal[x] is the one that is x - reach columns to the right of the tile's corner
     const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0 - reach;
+    // Far from the main diagonal 64 of them have one bucket: those are added up lane by lane until another one comes.
+    float run = 0.0f;
+    unsigned of = kMostBuckets;
+    auto finish = [&] {
+      if (of == kMostBuckets) return;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) run += __shfl_xor(run, o);
+      if (lane == 0) sums[wave][of] += run;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      run = 0.0f;
+      of = kMostBuckets;
+    };
     for (unsigned x0 = 0; x0 < reach + kCols; x0 += 64) {
       const unsigned x = x0 + lane;
       float sum = x < reach + kCols ? diagonal[wave][x] : 0.0f;
-      const unsigned u = bucket_of(b, (int64_t)(rel + x));
+      const unsigned u = bucket_of(b, border, (int64_t)(rel + x)), first = __builtin_amdgcn_readfirstlane(u);
+      if (__all(u == first)) {
+        if (first != of) finish();
+        of = first;
+        run += sum;
+        continue;
+      }
+      finish();
       // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
       const unsigned below = __shfl_up(u, 1), above = __shfl_down(u, 1);
       unsigned start = below != u && lane > 0 ? lane : 0;
-      if (__any(start != 0)) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const unsigned up = __shfl_up(start, o);
-          if (lane >= (unsigned)o && up > start) start = up;
-        }
+      for (int o = 1; o < 64; o <<= 1) {
+        const unsigned up = __shfl_up(start, o);
+        if (lane >= (unsigned)o && up > start) start = up;
       }
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -291,6 +332,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
       if (lane == 63 || above != u) sums[wave][u] += sum;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+    finish();
   }
   __syncthreads();
   for (unsigned u = threadIdx.x; u < buckets; u += kBlock) {
@@ -374,19 +416,24 @@ int check_strides(const char* what, const int64_t* stride, const Shape& s, bool 
 }
 
 // Enough wavefronts to fill the GPU, if that can be had: fewer rows for each first, then fewer batches, then fewer rows again.
-constexpr uint64_t kEnough = 4096;
-
-Cut cut_for(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
+#ifndef ENOUGH_F
+#define ENOUGH_F 4096
+#define ENOUGH_B 4096
+#define LEAST_ROWS 32
+#endif
+Cut cut_for(size_t B, size_t H, size_t Q, size_t K, bool own_positions, uint64_t enough) {
   Cut c;
   c.rows = kMostRows;
   while (c.rows / 2 >= Q && c.rows > kGroup) c.rows /= 2;
   c.batches = own_positions ? 1 : (unsigned)B;
   c.across = (unsigned)((K + kCols - 1) / kCols);
+  c.heads = 1;
+  c.parts = (unsigned)H;
   for (;;) {
     c.strips = (unsigned)((Q + c.rows - 1) / c.rows);
     c.chunks = (unsigned)((B + c.batches - 1) / c.batches);
-    if (c.tiles() * H >= kEnough) break;
-    if (c.rows > 32)
+    if (c.tiles() >= enough) break;
+    if (c.rows > LEAST_ROWS)
       c.rows /= 2;
     else if (c.batches > 1)
       c.batches = (c.batches + 1) / 2;
@@ -395,6 +442,24 @@ Cut cut_for(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
     else
       break;
   }
+  return c;
+}
+
+// Where a few queries need the same rows of the table for all heads, a wavefront takes several heads.
+Cut cut_for_bias(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
+  Cut c = cut_for(B, H, Q, K, own_positions, ENOUGH_F);
+  if (c.rows == kGroup)
+    while (c.heads < 8 && c.heads < H && c.tiles() >= 2 * ENOUGH_F) {
+      c.heads *= 2;
+      c.parts = (unsigned)((H + c.heads - 1) / c.heads);
+    }
+  return c;
+}
+
+// Of the gradient: the tiles of a head.
+Cut cut_for_sums(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
+  Cut c = cut_for(B, H, Q, K, own_positions, ENOUGH_B);
+  c.parts = 1;
   return c;
 }
 
@@ -411,7 +476,7 @@ extern "C" int pskv_relbias_bucket(int64_t rel, size_t buckets, uint64_t max_dis
   clear_error();
   Buckets b;
   const int rc = buckets_or_error(&b, buckets, max_distance, two_sided);
-  return rc ? rc : (int)bucket_of(b, rel);
+  return rc ? rc : (int)bucket_of(b, b.border, rel);
 }
 
 extern "C" int pskv_relbias(int device, void* stream, int type, const float* table, size_t buckets, size_t H,
@@ -440,14 +505,15 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
     if (!same && a < o + extent(out_stride, s, size) && o < a + extent(scores_stride, s, size))
       return set_error(PSKV_EINVAL, "out lies in the scores and is not the same tensor");
   }
+  const Cut cut = cut_for_bias(B, H, Q, K, q_at != nullptr);
+  if (cut.tiles() > kMostTiles) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
-  const Cut cut = cut_for(B, H, Q, K, q_at != nullptr);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     auto kernel = scores ? k_relbias<T, true> : k_relbias<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles() * H, kWaves, 1u << 22)), dim3(kBlock), 0,
-                       static_cast<hipStream_t>(stream), table, q_at, static_cast<const T*>(scores), static_cast<T*>(out), cut, s, b);
+    hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles(), kWaves, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), table,
+                       q_at, static_cast<const T*>(scores), static_cast<T*>(out), (unsigned)cut.tiles(), cut, s, b);
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
@@ -455,7 +521,7 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
 
 extern "C" size_t pskv_relbias_grad_room(size_t buckets, size_t H, size_t B, size_t Q, size_t K, int own_positions) {
   if (B == 0 || Q == 0 || K == 0 || B > (1u << 20) || Q > (1u << 20) || K > (1u << 30)) return 0;
-  return groups_of(cut_for(B, H, Q, K, own_positions != 0)) * buckets * H * sizeof(float);
+  return groups_of(cut_for_sums(B, H, Q, K, own_positions != 0)) * buckets * H * sizeof(float);
 }
 
 extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void* grad, const int64_t* grad_stride,
@@ -476,9 +542,9 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
     if (!grad) return set_error(PSKV_EINVAL, "null buffer");
     if ((rc = check_strides("grad", grad_stride, s, false))) return rc;
     for (int i = 0; i < 3; ++i) s.in[i] = (uint64_t)grad_stride[i];
-    cut = cut_for(B, H, Q, K, q_at != nullptr);
+    cut = cut_for_sums(B, H, Q, K, q_at != nullptr);
     groups = groups_of(cut);
-    if (groups > (1u << 23)) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
+    if (groups > kMostTiles / kBlock) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
     const size_t room = groups * buckets * H * sizeof(float);
     if (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3))
       return set_error(PSKV_EINVAL, "this gradient takes %zu bytes of working memory, %zu given", room, work ? work_bytes : (size_t)0);
@@ -491,7 +557,7 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       hipLaunchKernelGGL(k_relbias_sums<T>, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad),
-                         q_at, partial, (unsigned)buckets, cut, s, b);
+                         q_at, partial, (unsigned)buckets, (unsigned)cut.tiles(), cut, s, b);
     });
   hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(kBlock), 0, st, partial, (unsigned)buckets,
                      (unsigned)groups, (uint64_t)H, grad_table);

@@ -95,15 +95,20 @@ __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict_
     // the counts lie tile by tile: a thread's steps through them are 1,024 apart
     const unsigned all = tiles * bins, before = blockIdx.x * bins, hop = kSortBlock % bins;
     unsigned e = threadIdx.x % bins;
-#pragma unroll 8
-    for (unsigned i = threadIdx.x; i < all; i += kSortBlock) {
-      const unsigned c = counts[i];
-      if (c) {
-        atomicAdd(&total[e], c);
-        if (i < before) atomicAdd(&base[e], c);
+    constexpr unsigned kAhead = 8;
+    for (unsigned i0 = threadIdx.x; i0 < all; i0 += kAhead * kSortBlock) {
+      unsigned c[kAhead];
+#pragma unroll
+      for (unsigned a = 0; a < kAhead; ++a) c[a] = i0 + a * kSortBlock < all ? counts[i0 + a * kSortBlock] : 0;
+#pragma unroll
+      for (unsigned a = 0; a < kAhead; ++a) {
+        if (c[a]) {
+          atomicAdd(&total[e], c[a]);
+          if (i0 + a * kSortBlock < before) atomicAdd(&base[e], c[a]);
+        }
+        e += hop;
+        if (e >= bins) e -= bins;
       }
-      e += hop;
-      if (e >= bins) e -= bins;
     }
   }
   const unsigned bits = 32 - __builtin_clz(bins);
@@ -222,8 +227,8 @@ __global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ 
   }
 }
 
-// Eight answers are asked for at a time. A choice that is not here reads row 0, whose elements are replaced by zeros.
-template <typename T, bool ONE>
+// Past the caches where PAST: every answer is read once. Eight answers are asked for at a time. A choice that is not here reads row 0, whose elements are replaced by zeros.
+template <typename T, bool ONE, bool PAST>
 __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ rows, const int* __restrict__ place,
                                                           const float* __restrict__ weights, T* __restrict__ out, RowArgs a) {
   using Vec = typename Row<T>::Vec;
@@ -245,7 +250,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ r
           for (unsigned j = 0; j < N; ++j) {
             const uint64_t p = (uint64_t)(int64_t)at[j0 + j];
             here[j] = p < a.rows;
-            v[j] = *reinterpret_cast<const Vec*>(rows + (here[j] ? p : 0) * a.row_stride + c);
+            v[j] = get<PAST>(rows + (here[j] ? p : 0) * a.row_stride + c);
           }
 #pragma unroll
           for (unsigned j = 0; j < N; ++j) {
@@ -262,7 +267,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ r
         Vec v;
 #pragma unroll
         for (unsigned i = 0; i < W; ++i) v[i] = (T)sum[i];
-        *reinterpret_cast<Vec*>(to + c) = v;
+        put<PAST>(to + c, v);
       } else {
         const unsigned wide = (unsigned)(a.k - c);
         for (unsigned j = 0; j < a.choices; ++j) {
@@ -466,11 +471,15 @@ extern "C" int pskv_route_sum(int device, void* stream, int type, const void* ro
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   // (without rows there is no row 0 to read either)
   const RowArgs a = row_args(tokens, n_rows ? choices : 0, n_rows, k, out_stride, rows_stride, type, kRowBlock);
+  const bool past = (1 + choices) * tokens * k * size > kPastBytes;
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    auto kernel = a.lanes_log2 >= 6 ? k_route_sum<T, true> : k_route_sum<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(rows), place, weights, static_cast<T*>(out), a);
+    with_flag(past, [&](auto far) {
+      constexpr bool PAST = decltype(far)::value;
+      auto kernel = a.lanes_log2 >= 6 ? k_route_sum<T, true, PAST> : k_route_sum<T, false, PAST>;
+      hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+                         static_cast<hipStream_t>(stream), static_cast<const T*>(rows), place, weights, static_cast<T*>(out), a);
+    });
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
