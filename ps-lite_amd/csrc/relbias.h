@@ -30,23 +30,31 @@ struct Buckets {
   unsigned steps;   // borders in use
   unsigned two_sided;
   float log_exact, per_log;  // log2(exact), buckets per doubling of the distance
-  uint32_t border[kMostBuckets / 2];
+  uint32_t border[kMostBuckets / 2 + 1];  // 0, the least distances of the buckets that widen, the largest number
 };
 
-// The row of a relative position. The logarithm in float tells where to look (it is off by one at most), the borders decide;
-// near positions need neither. `border` is b.border, where it can be read fastest.
-PSKV_BOTH inline unsigned bucket_of(const Buckets& b, const uint32_t* border, int64_t rel) {
-  const uint64_t far = b.two_sided && rel > 0 ? (uint64_t)rel : rel < 0 ? 0 - (uint64_t)rel : 0;
-  const uint32_t d = far > kMostDistance ? (uint32_t)kMostDistance : (uint32_t)far;
-  unsigned row = d;
-  if (d >= b.exact) {
-    const float guess = (log2f((float)d) - b.log_exact) * b.per_log;
-    unsigned c = guess <= 0.0f ? 0 : guess >= (float)b.steps ? b.steps : (unsigned)guess;
-    while (c < b.steps && d >= border[c]) ++c;
-    while (c > 0 && d < border[c - 1]) --c;
-    row = b.exact + c;
-  }
-  return b.two_sided && rel > 0 ? b.side + row : row;
+// Relative positions beyond the largest distance, and tiles of them, have one bucket: positions are kept to 32 bits.
+PSKV_BOTH inline int32_t nearer(int64_t rel) {
+  const int64_t most = (int64_t)kMostDistance + 65536;
+  return rel > most ? (int32_t)most : rel < -most ? (int32_t)-most : (int32_t)rel;
+}
+
+// The row of a relative position. The logarithm in float tells where to look: its error, some 1e-6, times at most 11,400 buckets per
+// doubling is far below one, so the bucket is the one that it says or a neighbour, and the borders decide. `border` is b.border
+// with 0 in front and the largest number behind, where it can be read fastest.
+PSKV_BOTH inline unsigned bucket_of(const Buckets& b, const uint32_t* border, int32_t rel) {
+  const bool ahead = b.two_sided && rel > 0;
+  const uint32_t d = ahead ? (uint32_t)rel : rel < 0 ? 0 - (uint32_t)rel : 0;
+#ifdef __HIP_DEVICE_COMPILE__
+  const float log = __builtin_amdgcn_logf((float)d);
+#else
+  const float log = log2f((float)d);
+#endif
+  float guess = (log - b.log_exact) * b.per_log;
+  guess = guess > 0.0f ? guess : 0.0f;
+  const unsigned c = guess < (float)b.steps ? (unsigned)guess : b.steps;
+  const unsigned row = d < b.exact ? d : b.exact + c + (d >= border[c + 1] ? 1 : 0) - (d < border[c] ? 1 : 0);
+  return ahead ? b.side + row : row;
 }
 
 // A whole number of any length, for the few comparisons that a double cannot decide.
@@ -107,8 +115,10 @@ inline bool make_buckets(Buckets* b, uint64_t buckets, uint64_t max_distance, bo
     uint64_t d = (uint64_t)ceil(r - near);
     const uint64_t most = (uint64_t)floor(r + near);
     while (d <= most && !at_border(d, n, c, b->exact, max_distance)) ++d;
-    b->border[c - 1] = (uint32_t)d;
+    b->border[c] = (uint32_t)d;
   }
+  b->border[0] = 0;
+  b->border[n] = ~0u;
   return true;
 }
 

@@ -16,8 +16,6 @@ namespace {
 
 constexpr unsigned kBlock = 256;
 constexpr unsigned kWaves = kBlock / 64;
-constexpr unsigned kWide = 8;            // neighbouring columns of a lane
-constexpr unsigned kCols = 64 * kWide;   // of a wavefront
 constexpr unsigned kGroup = 8;           // rows that a wavefront asks for before it uses them
 constexpr unsigned kMostRows = 128;      // of a wavefront
 constexpr uint64_t kMostTiles = 1u << 31;
@@ -28,34 +26,35 @@ struct Shape {
   uint64_t in[3], out[3];  // strides of batch, head and row
 };
 
-// How a call is cut up: a wavefront takes `rows` rows of kCols columns, for `heads` heads and `batches` batches one after the other.
+// How a call is cut up: a wavefront takes `rows` rows of `cols` columns, for `heads` heads and `batches` batches one after the other.
 struct Cut {
-  unsigned rows, heads, batches;
+  unsigned cols, rows, heads, batches;
   unsigned across, strips, parts, chunks;  // how many there are of columns, rows, heads, batches
   uint64_t tiles() const { return (uint64_t)across * strips * parts * chunks; }
 };
 
-// Eight neighbouring elements, as they are in memory and as numbers.
-template <typename T>
-struct Eight {
-  static constexpr int kWords = 2 * (int)sizeof(T);
+// N neighbouring elements, as they are in memory and as numbers.
+template <typename T, unsigned N>
+struct Some {
+  static constexpr int kWords = (int)(N * sizeof(T) / 4);
   uint32_t word[kWords];
 
+  template <bool PAST>
   __device__ __forceinline__ void load(const T* p) {
     typedef uint32_t Quad __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int q = 0; q < kWords / 4; ++q) {
-      const Quad v = __builtin_bit_cast(Quad, reinterpret_cast<const typename Row<T>::Vec*>(p)[q]);
+      const Quad v = __builtin_bit_cast(Quad, get<PAST>(p + q * Row<T>::kWide));
 #pragma unroll
       for (int i = 0; i < 4; ++i) word[4 * q + i] = v[i];
     }
   }
-  // n (up to 8) of them, zeros behind them.
+  // n (up to N) of them, zeros behind them.
   __device__ __forceinline__ void few(const T* p, unsigned n) {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) word[i] = 0;
 #pragma unroll
-    for (unsigned i = 0; i < 8; ++i)
+    for (unsigned i = 0; i < N; ++i)
       if (i < n) {
         if constexpr (sizeof(T) == 4)
           word[i] = __builtin_bit_cast(uint32_t, p[i]);
@@ -63,7 +62,7 @@ struct Eight {
           word[i / 2] |= (uint32_t)__builtin_bit_cast(unsigned short, p[i]) << (i & 1 ? 16 : 0);
       }
   }
-  // The elements from `off` (up to 8) on, zeros behind them: what a lane at the end of a row needs that has loaded the last eight.
+  // The elements from `off` (up to N) on, zeros behind them: what a lane at the end of a row needs that has loaded the last N.
   __device__ __forceinline__ void skip(unsigned off) {
     constexpr int kHalf = sizeof(T) == 2 ? 1 : 0;
     if (kHalf) {
@@ -88,23 +87,31 @@ struct Eight {
   }
 };
 
-// Rounds eight numbers and stores the first n of them.
-template <typename T>
-__device__ __forceinline__ void store_eight(T* p, const float (&y)[8], unsigned n) {
-  constexpr int kSome = Row<T>::kWide;
-  if (n == 8) {
+// Rounds N numbers and stores the first n of them.
+template <bool PAST, unsigned N, typename T>
+__device__ __forceinline__ void store_some(T* p, const float (&y)[N], unsigned n) {
+  constexpr unsigned kSome = Row<T>::kWide;
+  T e[N];
 #pragma unroll
-    for (int q = 0; q < 8 / kSome; ++q) {
+  for (unsigned i = 0; i < N; ++i) e[i] = (T)y[i];
+  if (n == N) {
+#pragma unroll
+    for (unsigned q = 0; q < N / kSome; ++q) {
       typename Row<T>::Vec v;
 #pragma unroll
-      for (int i = 0; i < kSome; ++i) v[i] = (T)y[q * kSome + i];
-      reinterpret_cast<typename Row<T>::Vec*>(p)[q] = v;
+      for (unsigned i = 0; i < kSome; ++i) v[i] = e[q * kSome + i];
+      put<PAST>(p + q * kSome, v);
     }
-  } else {
-#pragma unroll
-    for (unsigned i = 0; i < 7; ++i)
-      if (i < n) p[i] = (T)y[i];
+    return;
   }
+  // four, two and one of them
+  typedef T Two __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+  typedef T Four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  const unsigned done = N > 4 ? n & 4 : 0;
+  if (done) *reinterpret_cast<Four*>(p) = Four{e[0], e[1], e[2], e[3]};
+  const T a = done ? e[N - 4] : e[0], b = done ? e[N - 3] : e[1], c = done ? e[N - 2] : e[2];
+  if (n & 2) *reinterpret_cast<Two*>(p + done) = Two{a, b};
+  if (n & 1) p[done + (n & 2)] = n & 2 ? c : a;
 }
 
 // The lane below's `v`; lane 0 gets `first`.
@@ -113,37 +120,72 @@ __device__ __forceinline__ float from_below(float v, float first) {
                                                                0x138 /* wave_shr:1 */, 0xf, 0xf, false));
 }
 
-// A lane's part of the rows of a tile: columns c to c + 7, or what there is of them.
+// What the lane that CONTROL names has, 0 where there is none or the lane's row of 16 is not in ROWS.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, ROWS, 0xf, false);
+}
+
+// One step of a sum along the lanes that starts anew where `starts` is set: what has been summed up to the lane that CONTROL names
+// comes in, unless a start lies between.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ void sum_step(float& sum, uint32_t& starts) {
+  const float up = __builtin_bit_cast(float, dpp<CONTROL, ROWS>(__builtin_bit_cast(uint32_t, sum)));
+  const uint32_t there = dpp<CONTROL, ROWS>(starts);
+  sum = starts ? sum : sum + up;
+  starts |= there;
+}
+__device__ __forceinline__ float sum_along(float sum, uint32_t starts) {
+  sum_step<0x111 /* row_shr:1 */, 0xf>(sum, starts);
+  sum_step<0x112, 0xf>(sum, starts);
+  sum_step<0x114, 0xf>(sum, starts);
+  sum_step<0x118, 0xf>(sum, starts);
+  sum_step<0x142 /* row_bcast:15 */, 0xa>(sum, starts);
+  sum_step<0x143 /* row_bcast:31 */, 0xc>(sum, starts);
+  return sum;
+}
+
+// A lane's part of the rows of a tile: columns c to c + N - 1, or what there is of them.
+template <unsigned N>
 struct Span {
-  uint64_t at;     // where it loads: at c, or the last eight of the row
+  uint64_t at;     // where it loads: at c, or the last N of the row
   unsigned off;    // how many of those come before c
-  unsigned own;    // columns, 0 to 8
+  unsigned own;    // columns, 0 to N
   bool ends, few;  // the same for the wavefront: the row ends within its columns; it is shorter than a load
   __device__ __forceinline__ Span(uint64_t c0, unsigned lane, uint64_t K) {
-    const uint64_t c = c0 + lane * kWide;
-    ends = c0 + kCols > K;
-    few = K < kWide;
-    own = c >= K ? 0 : K - c < kWide ? (unsigned)(K - c) : kWide;
-    at = few || own == kWide ? c : K - kWide;
-    off = c - at < kWide ? (unsigned)(c - at) : kWide;
+    const uint64_t c = c0 + lane * N;
+    ends = c0 + 64 * N > K;
+    few = K < N;
+    own = c >= K ? 0 : K - c < N ? (unsigned)(K - c) : N;
+    at = few || own == N ? c : K - N;
+    off = c - at < N ? (unsigned)(c - at) : N;
   }
-  template <typename T>
-  __device__ __forceinline__ void load(Eight<T>& x, const T* row) const {
+  // kGroup rows, or the first n of them where not WHOLE. (All of them are asked for before any is touched.)
+  template <bool WHOLE, bool PAST, typename T>
+  __device__ __forceinline__ void load(Some<T, N> (&x)[kGroup], const T* row, uint64_t stride, unsigned n) const {
     if (few) {
-      x.few(row + at, own);
+#pragma unroll
+      for (unsigned r = 0; r < kGroup; ++r)
+        if (WHOLE || r < n) x[r].few(row + r * stride + at, own);
       return;
     }
-    x.load(row + at);
-    if (ends) x.skip(off);
+#pragma unroll
+    for (unsigned r = 0; r < kGroup; ++r)
+      if (WHOLE || r < n) x[r].template load<PAST>(row + r * stride + at);
+    if (ends) {
+#pragma unroll
+      for (unsigned r = 0; r < kGroup; ++r)
+        if (WHOLE || r < n) x[r].skip(off);
+    }
   }
 };
 
 // The tile of a wavefront.
 struct Tile {
-  uint64_t c0, r0;
+  uint64_t c0, r0;  // the first column and row
   unsigned head0, batch0, rows, heads, batches;
   __device__ __forceinline__ Tile(unsigned tile, const Cut& cut, const Shape& s) {
-    c0 = (uint64_t)(tile % cut.across) * kCols;
+    c0 = (uint64_t)(tile % cut.across) * cut.cols;
     tile /= cut.across;
     r0 = (uint64_t)(tile % cut.strips) * cut.rows;
     tile /= cut.strips;
@@ -157,88 +199,75 @@ struct Tile {
 
 // The borders in LDS, for the workgroup. (A barrier has to follow.)
 __device__ __forceinline__ void fetch_borders(uint32_t* to, const Buckets& b) {
-  for (unsigned c = threadIdx.x; c < b.steps; c += kBlock) to[c] = b.border[c];
+  for (unsigned c = threadIdx.x; c < b.steps + 2; c += kBlock) to[c] = b.border[c];
 }
 
-// A tile of the bias. Row i's bias is row i - 1's, moved one column to the right, so eight rows further down a lane needs what
-// the lane below had: eight values of a lane's own and eight that it is handed serve eight rows, and nothing is looked up
-// but the tile's first row and, for lane 0, its first column, which waits in LDS.
-template <typename T, bool SCORES>
+// The bias, eight rows to a wavefront, of 16 bytes of columns to a lane, of one head after the other. A row's bias is that of the row
+// above, moved one column to the right, so what eight rows need is the first row's and the eight columns to the left of it, which
+// the lanes below have.
+template <typename T, bool SCORES, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_relbias(const float* __restrict__ table, const int64_t* __restrict__ q_at,
                                                      const T* scores, T* out, unsigned tiles, Cut cut, Shape s, Buckets b) {
-  __shared__ uint32_t border[kMostBuckets / 2];
-  __shared__ float left[kWaves][kMostRows];  // diagonals -1, -2, ... of the wavefront's tile
+  constexpr unsigned N = Row<T>::kWide;
+  __shared__ uint32_t border[kMostBuckets / 2 + 1];
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   fetch_borders(border, b);
   __syncthreads();
   for (unsigned tile = blockIdx.x * kWaves + wave; tile < tiles; tile += gridDim.x * kWaves) {
     const Tile t(tile, cut, s);
-    const Span span(t.c0, lane, s.K);
-    const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0;
-    const unsigned reach = (t.rows + kGroup - 1) / kGroup * kGroup;
-    unsigned row[kWide], below[kMostRows / 64];  // of the table, for the tile's first row and its first column
+    const Span<N> span(t.c0, lane, s.K);
+    const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0));
+    unsigned row[N];  // of the table
 #pragma unroll
-    for (unsigned k = 0; k < kWide; ++k) row[k] = bucket_of(b, border, (int64_t)(rel + lane * kWide + k)) * (unsigned)s.H;
-#pragma unroll
-    for (unsigned q = 0; q < kMostRows / 64; ++q)
-      below[q] = q * 64 < reach ? bucket_of(b, border, (int64_t)(rel - 1 - q * 64 - lane)) * (unsigned)s.H : 0;
-    const T* from0 = SCORES ? scores + t.batch0 * s.in[0] + t.head0 * s.in[1] + t.r0 * s.in[2] : nullptr;
-    T* to0 = out + t.batch0 * s.out[0] + t.head0 * s.out[1] + t.r0 * s.out[2] + t.c0 + lane * kWide;
+    for (unsigned k = 0; k < N; ++k) row[k] = bucket_of(b, border, rel + (int)(lane * N + k)) * (unsigned)s.H;
+    // the eight columns to the left of the tile: lanes 0 to 7 have one each
+    const unsigned left = bucket_of(b, border, rel - (int)kGroup + (int)(lane & (kGroup - 1))) * (unsigned)s.H;
     for (unsigned h = 0; h < t.heads; ++h) {
-      const float* column = table + t.head0 + h;
-      float v[kWide], next[kWide];
+      const uint64_t head = t.head0 + h;
+      const T* from = SCORES ? scores + t.batch0 * s.in[0] + head * s.in[1] + t.r0 * s.in[2] : nullptr;
+      T* to = out + t.batch0 * s.out[0] + head * s.out[1] + t.r0 * s.out[2] + t.c0 + lane * N;
+      auto group = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        Some<T, N> x[kGroup];
+        if (SCORES) span.template load<WHOLE, PAST>(x, from, s.in[2], t.rows);
+        float v[kGroup + N];  // v[kGroup + k]: of the first row's column k
+        const float corner = table[left + head];
 #pragma unroll
-      for (unsigned k = 0; k < kWide; ++k) v[k] = column[row[k]];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (unsigned k = 0; k < N; ++k) v[kGroup + k] = table[row[k] + head];
+        // handed up from the lane below, N columns at a time
 #pragma unroll
-      for (unsigned q = 0; q < kMostRows / 64; ++q)
-        if (q * 64 < reach) left[wave][q * 64 + lane] = column[below[q]];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const T* from = SCORES ? from0 + h * s.in[1] : nullptr;
-      T* to = to0 + h * s.out[1];
-      for (unsigned i = 0; i < t.rows; i += kGroup) {
+        for (int k = kGroup - 1; k >= 0; --k)
+          v[k] = from_below(v[k + N], __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, corner), k)));
 #pragma unroll
-        for (unsigned k = 0; k < kWide; ++k) next[k] = from_below(v[k], left[wave][i + kGroup - 1 - k]);
-        auto group = [&](auto whole) {
-          for (unsigned n = 0; n < t.batches; ++n) {
-            Eight<T> x[kGroup];
+        for (unsigned r = 0; r < kGroup; ++r) {
+          if (!WHOLE && r >= t.rows) continue;
+          float y[N];
 #pragma unroll
-            for (unsigned r = 0; r < kGroup; ++r)
-              if (SCORES && (whole || i + r < t.rows)) span.load(x[r], from + n * s.in[0] + (uint64_t)(i + r) * s.in[2]);
-#pragma unroll
-            for (unsigned r = 0; r < kGroup; ++r) {
-              if (!whole && i + r >= t.rows) continue;
-              float y[kWide];
-#pragma unroll
-              for (unsigned k = 0; k < kWide; ++k) {
-                y[k] = k >= r ? v[k - r] : next[kWide + k - r];
-                if (SCORES) y[k] = x[r].at(k) + y[k];
-              }
-              store_eight(to + n * s.out[0] + (uint64_t)(i + r) * s.out[2], y, span.own);
-            }
-          }
-        };
-        if (i + kGroup <= t.rows)
-          group(std::true_type());
-        else
-          group(std::false_type());
-#pragma unroll
-        for (unsigned k = 0; k < kWide; ++k) v[k] = next[k];
-      }
+          for (unsigned k = 0; k < N; ++k) y[k] = SCORES ? x[r].at(k) + v[kGroup + k - r] : v[kGroup + k - r];
+          store_some<PAST>(to + r * s.out[2], y, span.own);
+        }
+      };
+      if (t.rows == kGroup)
+        group(std::true_type());
+      else
+        group(std::false_type());
     }
   }
 }
 
 // --- the gradient ------------------------------------------------------------------------------------------------
 
-// The same tiles the other way round: rows are summed over the batch, then along the diagonals, which move up one lane every
+constexpr unsigned kWide = 8;           // neighbouring columns of a lane
+constexpr unsigned kCols = 64 * kWide;  // of a wavefront
+
+// The same the other way round: rows are summed over the batch, then along the diagonals, which move up one lane every
 // eight rows; those that leave lane 63 and those that are there in the end are summed by bucket, 64 neighbouring diagonals
 // at a time. Every sum has one order. partial[head][bucket][workgroup of the head].
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ grad, const int64_t* __restrict__ q_at,
                                                           float* __restrict__ partial, unsigned buckets, unsigned tiles,
                                                           Cut cut, Shape s, Buckets b) {
-  __shared__ uint32_t border[kMostBuckets / 2];
+  __shared__ uint32_t border[kMostBuckets / 2 + 1];
   __shared__ float diagonal[kWaves][kMostRows + kCols];
   __shared__ float sums[kWaves][kMostBuckets];
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -249,21 +278,20 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
   __syncthreads();
   if (tile < tiles) {
     const Tile t(tile, cut, s);  // (of any head: cut.parts is 1)
-    const Span span(t.c0, lane, s.K);
+    const Span<kWide> span(t.c0, lane, s.K);
     const T* from = grad + t.batch0 * s.in[0] + head * s.in[1] + t.r0 * s.in[2];
     const unsigned reach = (t.rows + kGroup - 1) / kGroup * kGroup;
     float high[kWide] = {};  // of the diagonals that begin the group's first row
     for (unsigned i = 0; i < t.rows; i += kGroup) {
       float sum[kGroup][kWide] = {};
       auto group = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
         for (unsigned n = 0; n < t.batches; ++n) {
-          Eight<T> x[kGroup];
+          Some<T, kWide> x[kGroup];
+          span.template load<WHOLE, PAST>(x, from + n * s.in[0] + i * s.in[2], s.in[2], t.rows - i);
 #pragma unroll
           for (unsigned r = 0; r < kGroup; ++r)
-            if (whole || i + r < t.rows) span.load(x[r], from + n * s.in[0] + (uint64_t)(i + r) * s.in[2]);
-#pragma unroll
-          for (unsigned r = 0; r < kGroup; ++r)
-            if (whole || i + r < t.rows)
+            if (WHOLE || i + r < t.rows)
 #pragma unroll
               for (unsigned k = 0; k < kWide; ++k) sum[r][k] += x[r].at(k);
         }
@@ -292,15 +320,14 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     for (unsigned k = 0; k < kWide; ++k) diagonal[wave][lane * kWide + k] = high[k];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // diagonal[x] is the one that is x - reach columns to the right of the tile's corner
-    const uint64_t rel = (uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0 - reach;
+    const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0 - reach));
     // Far from the main diagonal 64 of them have one bucket: those are added up lane by lane until another one comes.
     float run = 0.0f;
     unsigned of = kMostBuckets;
     auto finish = [&] {
       if (of == kMostBuckets) return;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) run += __shfl_xor(run, o);
-      if (lane == 0) sums[wave][of] += run;
+      run = sum_along(run, 0);
+      if (lane == 63) sums[wave][of] += run;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       run = 0.0f;
       of = kMostBuckets;
@@ -308,7 +335,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     for (unsigned x0 = 0; x0 < reach + kCols; x0 += 64) {
       const unsigned x = x0 + lane;
       float sum = x < reach + kCols ? diagonal[wave][x] : 0.0f;
-      const unsigned u = bucket_of(b, border, (int64_t)(rel + x)), first = __builtin_amdgcn_readfirstlane(u);
+      const unsigned u = bucket_of(b, border, rel + (int)x), first = __builtin_amdgcn_readfirstlane(u);
       if (__all(u == first)) {
         if (first != of) finish();
         of = first;
@@ -317,18 +344,8 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
       }
       finish();
       // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
-      const unsigned below = __shfl_up(u, 1), above = __shfl_down(u, 1);
-      unsigned start = below != u && lane > 0 ? lane : 0;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const unsigned up = __shfl_up(start, o);
-        if (lane >= (unsigned)o && up > start) start = up;
-      }
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const float up = __shfl_up(sum, o);
-        if (lane >= start + o) sum += up;
-      }
+      const unsigned below = dpp<0x138 /* wave_shr:1 */, 0xf>(u), above = dpp<0x130 /* wave_shl:1 */, 0xf>(u);
+      sum = sum_along(sum, lane == 0 || below != u ? 1 : 0);
       if (lane == 63 || above != u) sums[wave][u] += sum;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -343,23 +360,15 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
   }
 }
 
-__global__ __launch_bounds__(kBlock) void k_relbias_join(const float* __restrict__ partial, unsigned buckets, unsigned slots,
+__global__ __launch_bounds__(64) void k_relbias_join(const float* __restrict__ partial, unsigned buckets, unsigned slots,
                                                           uint64_t H, float* __restrict__ grad_table) {
-  __shared__ float red[kBlock / 64];
   const uint64_t head = blockIdx.y;
   const unsigned u = blockIdx.x;
   const float* from = partial + (head * buckets + u) * slots;
   float sum = 0.0f;
-  for (unsigned i = threadIdx.x; i < slots; i += kBlock) sum += from[i];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float t = red[0];
-    for (unsigned w = 1; w < kBlock / 64; ++w) t += red[w];
-    grad_table[(uint64_t)u * H + head] = t;
-  }
+  for (unsigned i = threadIdx.x; i < slots; i += 64) sum += from[i];
+  sum = sum_along(sum, 0);
+  if (threadIdx.x == 63) grad_table[(uint64_t)u * H + head] = sum;
 }
 
 // --- the host's checks -------------------------------------------------------------------------------------------
@@ -415,25 +424,41 @@ int check_strides(const char* what, const int64_t* stride, const Shape& s, bool 
   return PSKV_OK;
 }
 
-// Enough wavefronts to fill the GPU, if that can be had: fewer rows for each first, then fewer batches, then fewer rows again.
-#ifndef ENOUGH_F
-#define ENOUGH_F 4096
-#define ENOUGH_B 4096
-#define LEAST_ROWS 32
-#endif
-Cut cut_for(size_t B, size_t H, size_t Q, size_t K, bool own_positions, uint64_t enough) {
-  Cut c;
+constexpr uint64_t kFilled = 2048;  // wavefronts that fill the GPU
+
+// Of the bias: a wavefront takes eight rows, so that those at work stay close together in memory. Where a few queries need the same
+// rows of the table for all heads, it takes several heads, as long as the GPU is filled.
+Cut cut_for_bias(size_t B, size_t H, size_t Q, size_t K, size_t size) {
+  Cut c{};
+  c.cols = 64 * 16 / (unsigned)size;
+  c.rows = kGroup;
+  c.across = (unsigned)((K + c.cols - 1) / c.cols);
+  c.strips = (unsigned)((Q + c.rows - 1) / c.rows);
+  c.batches = c.heads = 1;
+  c.chunks = (unsigned)B;
+  c.parts = (unsigned)H;
+  while (c.heads < 8 && c.heads < H && c.strips == 1 && c.tiles() >= 2 * kFilled) {
+    c.heads *= 2;
+    c.parts = (unsigned)((H + c.heads - 1) / c.heads);
+  }
+  return c;
+}
+
+// Of the gradient: the tiles of a head. Enough wavefronts to fill the GPU, if that can be had: fewer rows for each first, then fewer
+// batches, then fewer rows again (64 rows as long as there are batches to share out: 16 x 2048 x 2048 bf16 28 us, from 32 rows on 32).
+Cut cut_for_sums(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
+  Cut c{};
+  c.cols = kCols;
   c.rows = kMostRows;
   while (c.rows / 2 >= Q && c.rows > kGroup) c.rows /= 2;
   c.batches = own_positions ? 1 : (unsigned)B;
   c.across = (unsigned)((K + kCols - 1) / kCols);
-  c.heads = 1;
-  c.parts = (unsigned)H;
+  c.heads = c.parts = 1;
   for (;;) {
     c.strips = (unsigned)((Q + c.rows - 1) / c.rows);
     c.chunks = (unsigned)((B + c.batches - 1) / c.batches);
-    if (c.tiles() >= enough) break;
-    if (c.rows > LEAST_ROWS)
+    if (c.tiles() * H >= kFilled) break;
+    if (c.rows > 64)
       c.rows /= 2;
     else if (c.batches > 1)
       c.batches = (c.batches + 1) / 2;
@@ -442,24 +467,6 @@ Cut cut_for(size_t B, size_t H, size_t Q, size_t K, bool own_positions, uint64_t
     else
       break;
   }
-  return c;
-}
-
-// Where a few queries need the same rows of the table for all heads, a wavefront takes several heads.
-Cut cut_for_bias(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
-  Cut c = cut_for(B, H, Q, K, own_positions, ENOUGH_F);
-  if (c.rows == kGroup)
-    while (c.heads < 8 && c.heads < H && c.tiles() >= 2 * ENOUGH_F) {
-      c.heads *= 2;
-      c.parts = (unsigned)((H + c.heads - 1) / c.heads);
-    }
-  return c;
-}
-
-// Of the gradient: the tiles of a head.
-Cut cut_for_sums(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
-  Cut c = cut_for(B, H, Q, K, own_positions, ENOUGH_B);
-  c.parts = 1;
   return c;
 }
 
@@ -476,7 +483,7 @@ extern "C" int pskv_relbias_bucket(int64_t rel, size_t buckets, uint64_t max_dis
   clear_error();
   Buckets b;
   const int rc = buckets_or_error(&b, buckets, max_distance, two_sided);
-  return rc ? rc : (int)bucket_of(b, b.border, rel);
+  return rc ? rc : (int)bucket_of(b, b.border, nearer(rel));
 }
 
 extern "C" int pskv_relbias(int device, void* stream, int type, const float* table, size_t buckets, size_t H,
@@ -505,15 +512,18 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
     if (!same && a < o + extent(out_stride, s, size) && o < a + extent(scores_stride, s, size))
       return set_error(PSKV_EINVAL, "out lies in the scores and is not the same tensor");
   }
-  const Cut cut = cut_for_bias(B, H, Q, K, q_at != nullptr);
+  const Cut cut = cut_for_bias(B, H, Q, K, type_bytes(type));
   if (cut.tiles() > kMostTiles) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    auto kernel = scores ? k_relbias<T, true> : k_relbias<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles(), kWaves, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream), table,
-                       q_at, static_cast<const T*>(scores), static_cast<T*>(out), (unsigned)cut.tiles(), cut, s, b);
+    with_flag(B * H * Q * K * sizeof(T) * (scores ? 2 : 1) > kPastBytes, [&](auto far) {
+      constexpr bool PAST = decltype(far)::value;
+      auto kernel = scores ? k_relbias<T, true, PAST> : k_relbias<T, false, PAST>;
+      hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles(), kWaves, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream),
+                         table, q_at, static_cast<const T*>(scores), static_cast<T*>(out), (unsigned)cut.tiles(), cut, s, b);
+    });
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
@@ -556,10 +566,12 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
   if (any)
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      hipLaunchKernelGGL(k_relbias_sums<T>, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad),
+      // (of several gradients of 83 MB in turn, 31 us each, some is still in the memory-side cache, 34 past it; of 134 MB 32 and 29)
+      auto kernel = B * H * Q * K * sizeof(T) > kPastBytes / 2 ? k_relbias_sums<T, true> : k_relbias_sums<T, false>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad),
                          q_at, partial, (unsigned)buckets, (unsigned)cut.tiles(), cut, s, b);
     });
-  hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(kBlock), 0, st, partial, (unsigned)buckets,
+  hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(64), 0, st, partial, (unsigned)buckets,
                      (unsigned)groups, (uint64_t)H, grad_table);
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;

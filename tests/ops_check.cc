@@ -29,7 +29,7 @@ int main() {
         printf("refused\n");
         continue;
       }
-      for (unsigned c = 0; c < b.steps; ++c) printf("%u ", b.border[c]);
+      for (unsigned c = 1; c <= b.steps; ++c) printf("%u ", b.border[c]);
       printf("\n");
     } else if (!strcmp(what, "philox")) {
       uint32_t x[6];
