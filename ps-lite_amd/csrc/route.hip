@@ -113,19 +113,24 @@ __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict_
   }
   const unsigned bits = 32 - __builtin_clz(bins);
   const uint64_t before = (1ull << lane) - 1;
+  uint64_t same[ITEMS];  // the lanes of the same bin
+#pragma unroll
+  for (unsigned s = 0; s < ITEMS; ++s) same[s] = ~0ull;
+  for (unsigned b = 0; b < bits; ++b) {
+#pragma unroll
+    for (unsigned s = 0; s < ITEMS; ++s) {
+      const int bit = (int)(bin[s] << (31 - b)) >> 31;  // 0 or all ones
+      const uint64_t ones = __ballot(bit != 0);
+      same[s] &= ~(ones ^ (uint64_t)(int64_t)bit);
+    }
+  }
 #pragma unroll
   for (unsigned s = 0; s < ITEMS; ++s) {
-    uint64_t same = ~0ull;
-    for (unsigned b = 0; b < bits; ++b) {
-      const bool one = (bin[s] >> b) & 1;
-      const uint64_t ones = __ballot(one);
-      same &= one ? ones : ~ones;
-    }
     if (bin[s] < bins) {
       const unsigned so_far = mine[wave][bin[s]];
-      rank[s] = so_far + __popcll(same & before);
+      rank[s] = so_far + __popcll(same[s] & before);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if ((same >> lane) == 1) mine[wave][bin[s]] = (unsigned short)(so_far + __popcll(same));
+      if ((same[s] >> lane) == 1) mine[wave][bin[s]] = (unsigned short)(so_far + __popcll(same[s]));
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -199,7 +204,7 @@ __device__ __forceinline__ uint64_t token_of(uint64_t t) {
   return (uint64_t)__builtin_amdgcn_readfirstlane((int)(t >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)t);
 }
 
-template <typename T, bool ONE>
+template <typename T, bool ONE, bool PAST>
 __global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ x, const int* __restrict__ place,
                                                            T* __restrict__ out, RowArgs a) {
   using Vec = typename Row<T>::Vec;
@@ -211,10 +216,10 @@ __global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ 
     const int* at = place + t * a.choices;
     for (uint64_t c = (uint64_t)(threadIdx.x & (lanes - 1)) * W; c < a.k; c += (uint64_t)lanes * W) {
       if (c + W <= a.k) {
-        const Vec v = *reinterpret_cast<const Vec*>(from + c);
+        const Vec v = get<false>(from + c);
         for (unsigned j = 0; j < a.choices; ++j) {
           const uint64_t p = (uint64_t)(int64_t)at[j];
-          if (p < a.rows) *reinterpret_cast<Vec*>(out + p * a.row_stride + c) = v;
+          if (p < a.rows) put<PAST>(out + p * a.row_stride + c, v);
         }
       } else {
         for (unsigned j = 0; j < a.choices; ++j) {
@@ -227,7 +232,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ 
   }
 }
 
-// Past the caches where PAST: every answer is read once. Eight answers are asked for at a time. A choice that is not here reads row 0, whose elements are replaced by zeros.
+// Eight answers are asked for at a time. A choice that is not here reads row 0, whose elements are replaced by zeros.
 template <typename T, bool ONE, bool PAST>
 __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ rows, const int* __restrict__ place,
                                                           const float* __restrict__ weights, T* __restrict__ out, RowArgs a) {
@@ -290,7 +295,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ r
 // token's gradient, up to kKept vectors of it, for all choices, and asks for the next answer before it uses one.
 constexpr unsigned kKept = 4;
 
-template <typename T, bool ONE>
+template <typename T, bool ONE, bool PAST>
 __global__ __launch_bounds__(kRowBlock) void k_route_sum_grad(const T* __restrict__ grad, const T* __restrict__ rows,
                                                                const int* __restrict__ place,
                                                                const float* __restrict__ weights, T* __restrict__ grad_rows,
@@ -324,7 +329,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum_grad(const T* __restric
         for (uint64_t c0 = lane * W; c0 < whole; c0 += kKept * wide) {
 #pragma unroll
           for (unsigned q = 0; q < kKept; ++q)
-            if (c0 + q * wide < whole) v[q] = *reinterpret_cast<const Vec*>(from + c0 + q * wide);
+            if (c0 + q * wide < whole) v[q] = get<PAST>(from + c0 + q * wide);
           if (!kept) {
 #pragma unroll
             for (unsigned q = 0; q < kKept; ++q)
@@ -339,7 +344,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum_grad(const T* __restric
                 sum = __builtin_fmaf((float)d[q][i], (float)v[q][i], sum);
                 o[i] = (T)(f * (float)d[q][i]);
               }
-              *reinterpret_cast<Vec*>(to + c0 + q * wide) = o;
+              put<PAST>(to + c0 + q * wide, o);
             }
         }
         for (uint64_t i = whole + lane; i < a.k; i += lanes) {
@@ -451,9 +456,12 @@ extern "C" int pskv_route_rows(int device, void* stream, int type, const void* x
   const RowArgs a = row_args(tokens, choices, n_rows, k, x_stride, rows_stride, type, lanes_of(tokens));
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    auto kernel = a.lanes_log2 >= 6 ? k_route_rows<T, true> : k_route_rows<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(x), place, static_cast<T*>(rows), a);
+    with_flag((1 + choices) * tokens * k * size > kPastBytes, [&](auto far) {
+      constexpr bool PAST = decltype(far)::value;
+      auto kernel = a.lanes_log2 >= 6 ? k_route_rows<T, true, PAST> : k_route_rows<T, false, PAST>;
+      hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+                         static_cast<hipStream_t>(stream), static_cast<const T*>(x), place, static_cast<T*>(rows), a);
+    });
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
@@ -475,10 +483,9 @@ extern "C" int pskv_route_sum(int device, void* stream, int type, const void* ro
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   // (without rows there is no row 0 to read either)
   const RowArgs a = row_args(tokens, n_rows ? choices : 0, n_rows, k, out_stride, rows_stride, type, lanes_of(tokens));
-  const bool past = (1 + choices) * tokens * k * size > kPastBytes;
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    with_flag(past, [&](auto far) {
+    with_flag((1 + choices) * tokens * k * size > kPastBytes, [&](auto far) {
       constexpr bool PAST = decltype(far)::value;
       auto kernel = a.lanes_log2 >= 6 ? k_route_sum<T, true, PAST> : k_route_sum<T, false, PAST>;
       hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
@@ -510,10 +517,13 @@ extern "C" int pskv_route_sum_grad(int device, void* stream, int type, const voi
   const RowArgs a = row_args(tokens, choices, n_rows, k, grad_stride, rows_stride, type, 64);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    auto kernel = a.lanes_log2 >= 6 ? k_route_sum_grad<T, true> : k_route_sum_grad<T, false>;
-    hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
-                       static_cast<hipStream_t>(stream), static_cast<const T*>(grad), static_cast<const T*>(rows), place, weights,
-                       static_cast<T*>(grad_rows), (uint64_t)grad_rows_stride, grad_weights, a);
+    with_flag((1 + 2 * choices) * tokens * k * size > kPastBytes, [&](auto far) {
+      constexpr bool PAST = decltype(far)::value;
+      auto kernel = a.lanes_log2 >= 6 ? k_route_sum_grad<T, true, PAST> : k_route_sum_grad<T, false, PAST>;
+      hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+                         static_cast<hipStream_t>(stream), static_cast<const T*>(grad), static_cast<const T*>(rows), place, weights,
+                         static_cast<T*>(grad_rows), (uint64_t)grad_rows_stride, grad_weights, a);
+    });
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
