@@ -202,7 +202,7 @@ __device__ __forceinline__ void fetch_borders(uint32_t* to, const Buckets& b) {
   for (unsigned c = threadIdx.x; c < b.steps + 2; c += kBlock) to[c] = b.border[c];
 }
 
-// The bias, eight rows to a wavefront, of 16 bytes of columns to a lane, of one head after the other. A row's bias is that of the row
+// The bias, eight rows to a wavefront, of 16 bytes of columns to a lane, of one head. A row's bias is that of the row
 // above, moved one column to the right, so what eight rows need is the first row's and the eight columns to the left of it, which
 // the lanes below have.
 template <typename T, bool SCORES, bool PAST>
@@ -222,36 +222,72 @@ __global__ __launch_bounds__(kBlock) void k_relbias(const float* __restrict__ ta
     for (unsigned k = 0; k < N; ++k) row[k] = bucket_of(b, border, rel + (int)(lane * N + k)) * (unsigned)s.H;
     // the eight columns to the left of the tile: lanes 0 to 7 have one each
     const unsigned left = bucket_of(b, border, rel - (int)kGroup + (int)(lane & (kGroup - 1))) * (unsigned)s.H;
-    for (unsigned h = 0; h < t.heads; ++h) {
-      const uint64_t head = t.head0 + h;
-      const T* from = SCORES ? scores + t.batch0 * s.in[0] + head * s.in[1] + t.r0 * s.in[2] : nullptr;
-      T* to = out + t.batch0 * s.out[0] + head * s.out[1] + t.r0 * s.out[2] + t.c0 + lane * N;
-      auto group = [&](auto whole) {
-        constexpr bool WHOLE = decltype(whole)::value;
-        Some<T, N> x[kGroup];
-        if (SCORES) span.template load<WHOLE, PAST>(x, from, s.in[2], t.rows);
-        float v[kGroup + N];  // v[kGroup + k]: of the first row's column k
-        const float corner = table[left + head];
+    const uint64_t head = t.head0;
+    const T* from = SCORES ? scores + t.batch0 * s.in[0] + head * s.in[1] + t.r0 * s.in[2] : nullptr;
+    T* to = out + t.batch0 * s.out[0] + head * s.out[1] + t.r0 * s.out[2] + t.c0 + lane * N;
+    auto group = [&](auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      Some<T, N> x[kGroup];
+      if (SCORES) span.template load<WHOLE, PAST>(x, from, s.in[2], t.rows);
+      float v[kGroup + N];  // v[kGroup + k]: of the first row's column k
+      const float corner = table[left + head];
 #pragma unroll
-        for (unsigned k = 0; k < N; ++k) v[kGroup + k] = table[row[k] + head];
-        // handed up from the lane below, N columns at a time
+      for (unsigned k = 0; k < N; ++k) v[kGroup + k] = table[row[k] + head];
+      // handed up from the lane below, N columns at a time
 #pragma unroll
-        for (int k = kGroup - 1; k >= 0; --k)
-          v[k] = from_below(v[k + N], __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, corner), k)));
+      for (int k = kGroup - 1; k >= 0; --k)
+        v[k] = from_below(v[k + N], __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, corner), k)));
 #pragma unroll
-        for (unsigned r = 0; r < kGroup; ++r) {
-          if (!WHOLE && r >= t.rows) continue;
-          float y[N];
+      for (unsigned r = 0; r < kGroup; ++r) {
+        if (!WHOLE && r >= t.rows) continue;
+        float y[N];
 #pragma unroll
-          for (unsigned k = 0; k < N; ++k) y[k] = SCORES ? x[r].at(k) + v[kGroup + k - r] : v[kGroup + k - r];
-          store_some<PAST>(to + r * s.out[2], y, span.own);
-        }
-      };
-      if (t.rows == kGroup)
-        group(std::true_type());
-      else
-        group(std::false_type());
-    }
+        for (unsigned k = 0; k < N; ++k) y[k] = SCORES ? x[r].at(k) + v[kGroup + k - r] : v[kGroup + k - r];
+        store_some<PAST>(to + r * s.out[2], y, span.own);
+      }
+    };
+    if (t.rows == kGroup)
+      group(std::true_type());
+    else
+      group(std::false_type());
+  }
+}
+
+// One query to a sequence: a wavefront takes the same columns of eight heads (or fewer), whose rows of the table are the same.
+template <typename T, bool SCORES>
+__global__ __launch_bounds__(kBlock) void k_relbias_step(const float* __restrict__ table, const int64_t* __restrict__ q_at,
+                                                          const T* scores, T* out, unsigned tiles, Cut cut, Shape s, Buckets b) {
+  constexpr unsigned N = Row<T>::kWide;
+  __shared__ uint32_t border[kMostBuckets / 2 + 1];
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  fetch_borders(border, b);
+  __syncthreads();
+  for (unsigned tile = blockIdx.x * kWaves + wave; tile < tiles; tile += gridDim.x * kWaves) {
+    const Tile t(tile, cut, s);
+    const Span<N> span(t.c0, lane, s.K);
+    auto heads = [&](auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      Some<T, N> x[kGroup];
+      if (SCORES)
+        span.template load<WHOLE, false>(x, scores + t.batch0 * s.in[0] + t.head0 * s.in[1], s.in[1], t.heads);
+      const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0));
+      unsigned row[N];
+#pragma unroll
+      for (unsigned k = 0; k < N; ++k) row[k] = bucket_of(b, border, rel + (int)(lane * N + k)) * (unsigned)s.H + t.head0;
+      T* to = out + t.batch0 * s.out[0] + t.head0 * s.out[1] + t.c0 + lane * N;
+#pragma unroll
+      for (unsigned h = 0; h < kGroup; ++h) {
+        if (!WHOLE && h >= t.heads) continue;
+        float y[N];
+#pragma unroll
+        for (unsigned k = 0; k < N; ++k) y[k] = SCORES ? x[h].at(k) + table[row[k] + h] : table[row[k] + h];
+        store_some<false>(to + h * s.out[1], y, span.own);
+      }
+    };
+    if (t.heads == kGroup)
+      heads(std::true_type());
+    else
+      heads(std::false_type());
   }
 }
 
@@ -426,8 +462,8 @@ int check_strides(const char* what, const int64_t* stride, const Shape& s, bool 
 
 constexpr uint64_t kFilled = 2048;  // wavefronts that fill the GPU
 
-// Of the bias: a wavefront takes eight rows, so that those at work stay close together in memory. Where a few queries need the same
-// rows of the table for all heads, it takes several heads, as long as the GPU is filled.
+// Of the bias: a wavefront takes eight rows, so that those at work stay close together in memory; eight heads where there is one query
+// only, fewer where that would not fill the GPU.
 Cut cut_for_bias(size_t B, size_t H, size_t Q, size_t K, size_t size) {
   Cut c{};
   c.cols = 64 * 16 / (unsigned)size;
@@ -437,7 +473,7 @@ Cut cut_for_bias(size_t B, size_t H, size_t Q, size_t K, size_t size) {
   c.batches = c.heads = 1;
   c.chunks = (unsigned)B;
   c.parts = (unsigned)H;
-  while (c.heads < 8 && c.heads < H && c.strips == 1 && c.tiles() >= 2 * kFilled) {
+  while (Q == 1 && c.heads < kGroup && c.heads < H && c.tiles() >= kFilled) {
     c.heads *= 2;
     c.parts = (unsigned)((H + c.heads - 1) / c.heads);
   }
@@ -518,12 +554,16 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    with_flag(B * H * Q * K * sizeof(T) * (scores ? 2 : 1) > kPastBytes, [&](auto far) {
-      constexpr bool PAST = decltype(far)::value;
-      auto kernel = scores ? k_relbias<T, true, PAST> : k_relbias<T, false, PAST>;
+    auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles(), kWaves, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream),
                          table, q_at, static_cast<const T*>(scores), static_cast<T*>(out), (unsigned)cut.tiles(), cut, s, b);
-    });
+    };
+    if (Q == 1)
+      launch(scores ? k_relbias_step<T, true> : k_relbias_step<T, false>);
+    else if (B * H * Q * K * sizeof(T) * (scores ? 2 : 1) > kPastBytes)
+      launch(scores ? k_relbias<T, true, true> : k_relbias<T, false, true>);
+    else
+      launch(scores ? k_relbias<T, true, false> : k_relbias<T, false, false>);
   });
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
