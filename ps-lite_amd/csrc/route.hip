@@ -20,8 +20,8 @@ constexpr unsigned kSortBlock = 1024;
 constexpr unsigned kSortWaves = kSortBlock / 64;
 constexpr unsigned kSortItems = 4;  // choices per lane; one where there are not more of them than lanes
 constexpr unsigned kSortTile = kSortBlock * kSortItems;
-// Up to so many tiles, every workgroup adds up the tiles' counts for itself; beyond, a launch of its own does.
-constexpr unsigned kSortFew = 128;
+// Up to so many counts, every workgroup adds up the tiles' for itself; beyond, a launch of its own does.
+constexpr uint64_t kSortFew = 32768;
 constexpr unsigned kSortBins = PSKV_ROUTE_MAX_EXPERTS + 1;  // the last one in use: choices that are not here
 
 template <typename I>
@@ -49,24 +49,37 @@ __global__ __launch_bounds__(kSortBlock) void k_route_count(const I* __restrict_
   for (unsigned e = threadIdx.x; e <= E; e += kSortBlock) counts[(uint64_t)blockIdx.x * (E + 1) + e] = hist[e];
 }
 
-// What every tile's choices of a bin follow, in place, and behind the last tile the bins' totals. A thread per bin, which
-// reads ahead: the tiles' counts do not depend on each other.
-__global__ __launch_bounds__(64) void k_route_scan(unsigned* __restrict__ counts, unsigned tiles, unsigned bins) {
-  const unsigned e = blockIdx.x * 64 + threadIdx.x;
-  if (e >= bins) return;
+// What every tile's choices of a bin follow, in place, and behind the last tile the bins' totals. A workgroup takes 64 bins, a lane
+// to each; its wavefronts share the tiles out, add up their parts, and go through them once more from where the parts before end.
+__global__ __launch_bounds__(kSortBlock) void k_route_scan(unsigned* __restrict__ counts, unsigned tiles, unsigned bins) {
+  __shared__ unsigned part[kSortWaves][64];
+  const unsigned wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e = blockIdx.x * 64 + lane;
+  const unsigned each = (tiles + kSortWaves - 1) / kSortWaves;
+  const unsigned first = wave * each < tiles ? wave * each : tiles, end = tiles - first < each ? tiles : first + each;
   constexpr unsigned kAhead = 16;
-  unsigned run = 0;
-  for (unsigned t0 = 0; t0 < tiles; t0 += kAhead) {
-    unsigned c[kAhead];
+  auto pass = [&](unsigned run, auto write) {
+    for (unsigned t0 = first; t0 < end; t0 += kAhead) {
+      unsigned c[kAhead];
 #pragma unroll
-    for (unsigned a = 0; a < kAhead; ++a) c[a] = t0 + a < tiles ? counts[(uint64_t)(t0 + a) * bins + e] : 0;
+      for (unsigned a = 0; a < kAhead; ++a) c[a] = t0 + a < end && e < bins ? counts[(uint64_t)(t0 + a) * bins + e] : 0;
 #pragma unroll
-    for (unsigned a = 0; a < kAhead; ++a) {
-      if (t0 + a < tiles) counts[(uint64_t)(t0 + a) * bins + e] = run;
-      run += c[a];
+      for (unsigned a = 0; a < kAhead; ++a) {
+        if (decltype(write)::value && t0 + a < end && e < bins) counts[(uint64_t)(t0 + a) * bins + e] = run;
+        run += c[a];
+      }
     }
+    return run;
+  };
+  part[wave][lane] = pass(0, std::false_type());
+  __syncthreads();
+  unsigned run = 0, all = 0;
+#pragma unroll
+  for (unsigned w = 0; w < kSortWaves; ++w) {
+    run += w < wave ? part[w][lane] : 0;
+    all += part[w][lane];
   }
-  counts[(uint64_t)tiles * bins + e] = run;
+  pass(run, std::true_type());
+  if (wave == 0 && e < bins) counts[(uint64_t)tiles * bins + e] = all;
 }
 
 // Places of a tile's choices. A wavefront owns neighbouring ones and takes them 64 at a time: lanes of the same bin find each
@@ -423,12 +436,12 @@ extern "C" int pskv_route_sort(int device, void* stream, const void* experts, in
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned tiles = n <= kSortTile ? 1u : (unsigned)((n + kSortTile - 1) / kSortTile);
-  const bool scanned = tiles > kSortFew;
+  const bool scanned = tiles * (E + 1) > kSortFew;
   unsigned* counts = static_cast<unsigned*>(work);
   auto go = [&](auto* e) {
     using I = std::remove_const_t<std::remove_pointer_t<decltype(e)>>;
     if (tiles > 1) hipLaunchKernelGGL(k_route_count<I>, dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts);
-    if (scanned) hipLaunchKernelGGL(k_route_scan, dim3((unsigned)E / 64 + 1), dim3(64), 0, st, counts, tiles, (unsigned)E + 1);
+    if (tiles > 1 && scanned) hipLaunchKernelGGL(k_route_scan, dim3((unsigned)E / 64 + 1), dim3(kSortBlock), 0, st, counts, tiles, (unsigned)E + 1);
     hipLaunchKernelGGL((n <= kSortBlock ? k_route_place<I, 1> : k_route_place<I, kSortItems>), dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts, tiles, scanned,
                        order, place, offsets);
   };
