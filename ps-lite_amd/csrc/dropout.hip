@@ -16,6 +16,7 @@ namespace {
 
 constexpr unsigned kBlock = 256;
 constexpr unsigned kDrawn = 8;  // columns that one draw serves
+constexpr uint64_t kMostDraws = (1ull << 31) - 2 * kBlock;  // of a launch
 
 template <typename T>
 __device__ __forceinline__ T keep(uint32_t word, bool high, unsigned least, T v, float scale) {
@@ -37,36 +38,34 @@ struct Divisor {
   }
 };
 
-template <typename T, bool FEW, bool PAST>
+// 16-bit types: a lane takes the 8 columns of a draw, 16 bytes. Indexes are those of draws.
+template <typename T, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_dropout(const T* x, T* out, const uint64_t* __restrict__ keys, uint64_t first,
-                                                     const uint64_t* __restrict__ step, uint64_t seed, uint64_t n, uint64_t k,
-                                                     uint64_t x_stride, uint64_t out_stride, unsigned least, float scale, Divisor per_row) {
-  using Vec = typename Row<T>::Vec;
+                                                     const uint64_t* __restrict__ step, uint64_t seed, uint32_t draws, uint32_t k,
+                                                     uint64_t x_stride, uint64_t out_stride, unsigned least, float scale,
+                                                     Divisor per_row) {
   constexpr unsigned W = Row<T>::kWide;
+  static_assert(W == kDrawn, "a vector is what a draw serves");
   if (step) seed += *step;
-  const uint64_t blocks = (k + kDrawn - 1) / kDrawn;
-  for (uint64_t at = (uint64_t)blockIdx.x * kBlock + threadIdx.x; at < n * blocks; at += (uint64_t)gridDim.x * kBlock) {
-    const uint64_t r = FEW ? per_row.of((uint32_t)at) : at / blocks, q = at - r * blocks;
-    const uint64_t key = keys ? keys[r] : first + r;
-    const uint64_t c = q * kDrawn;
-    const Drawn d = philox((uint32_t)key, (uint32_t)(key >> 32), (uint32_t)q, 0, (uint32_t)seed, (uint32_t)(seed >> 32));
-    const T* from = x + r * x_stride + c;
-    T* to = out + r * out_stride + c;
-    auto kept = [&](unsigned i, T v) { return keep(d.word[i / 2], i & 1, least, v, scale); };
-    if (k - c >= kDrawn) {
+  const uint32_t at = blockIdx.x * kBlock + threadIdx.x;
+  if (at >= draws) return;
+  const uint32_t r = per_row.of(at), q = at - r * per_row.d;
+  const uint64_t key = keys ? keys[r] : first + r;
+  const uint32_t c = q * kDrawn;
+  const Drawn d = philox((uint32_t)key, (uint32_t)(key >> 32), q, 0, (uint32_t)seed, (uint32_t)(seed >> 32));
+  const T* from = x + r * x_stride + c;
+  T* to = out + r * out_stride + c;
+  auto kept = [&](unsigned i, T v) { return keep(d.word[i / 2], i & 1, least, v, scale); };
+  if (k - c >= kDrawn) {
+    const typename Row<T>::Vec v = get<PAST>(from);
+    typename Row<T>::Vec o;
 #pragma unroll
-      for (unsigned i = 0; i < kDrawn; i += W) {
-        const Vec v = get<PAST>(from + i);
-        Vec o;
+    for (unsigned i = 0; i < kDrawn; ++i) o[i] = kept(i, v[i]);
+    put<PAST>(to, o);
+  } else {
 #pragma unroll
-        for (unsigned e = 0; e < W; ++e) o[e] = kept(i + e, v[e]);
-        put<PAST>(to + i, o);
-      }
-    } else {
-#pragma unroll
-      for (unsigned i = 0; i < kDrawn; ++i)
-        if (i < k - c) to[i] = kept(i, from[i]);
-    }
+    for (unsigned i = 0; i < kDrawn; ++i)
+      if (i < k - c) to[i] = kept(i, from[i]);
   }
 }
 
@@ -150,22 +149,28 @@ extern "C" int pskv_dropout(int device, void* stream, int type, const void* x, s
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  with_flag(2 * n * k * size > kPastBytes, [&](auto far) {
-    constexpr bool PAST = decltype(far)::value;
-    if (type == PSKV_F32 && n * blocks < (1ull << 31) - kBlock) {
-      hipLaunchKernelGGL(k_dropout_pairs<PAST>, dim3((unsigned)((n * blocks + kBlock - 1) / kBlock)), dim3(kBlock), 0, st,
-                         static_cast<const float*>(x), static_cast<float*>(out), keys, first, step, seed, (uint32_t)(2 * n * blocks),
-                         (uint32_t)k, (uint64_t)x_stride, (uint64_t)out_stride, least, scale, Divisor((uint32_t)(2 * blocks)));
-      return;
-    }
-    with_type(type, [&](auto* t) {
-      using T = std::remove_pointer_t<decltype(t)>;
-      auto kernel = n * blocks < (1ull << 32) ? k_dropout<T, true, PAST> : k_dropout<T, false, PAST>;
-      hipLaunchKernelGGL(kernel, dim3(grid_for(n * blocks, kBlock, 1u << 22)), dim3(kBlock), 0, st, static_cast<const T*>(x),
-                         static_cast<T*>(out), keys, first, step, seed, (uint64_t)n, (uint64_t)k, (uint64_t)x_stride,
-                         (uint64_t)out_stride, least, scale, Divisor((uint32_t)blocks));
+  // (a launch counts its draws in 31 bits)
+  const uint64_t most = kMostDraws / blocks;
+  for (uint64_t r0 = 0; r0 < n; r0 += most) {
+    const uint64_t rows = n - r0 < most ? n - r0 : most;
+    const uint32_t draws = (uint32_t)(rows * blocks);
+    const dim3 grid((draws + kBlock - 1) / kBlock);
+    const uint64_t* some = keys ? keys + r0 : nullptr;
+    with_flag(2 * n * k * size > kPastBytes, [&](auto far) {
+      constexpr bool PAST = decltype(far)::value;
+      with_type(type, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const T* from = static_cast<const T*>(x) + r0 * x_stride;
+        T* to = static_cast<T*>(out) + r0 * out_stride;
+        if constexpr (sizeof(T) == 4)
+          hipLaunchKernelGGL(k_dropout_pairs<PAST>, grid, dim3(kBlock), 0, st, from, to, some, first + r0, step, seed, 2 * draws,
+                             (uint32_t)k, (uint64_t)x_stride, (uint64_t)out_stride, least, scale, Divisor((uint32_t)(2 * blocks)));
+        else
+          hipLaunchKernelGGL((k_dropout<T, PAST>), grid, dim3(kBlock), 0, st, from, to, some, first + r0, step, seed, draws, (uint32_t)k,
+                             (uint64_t)x_stride, (uint64_t)out_stride, least, scale, Divisor((uint32_t)blocks));
+      });
     });
-  });
-  PSKV_HIP(hipGetLastError());
+    PSKV_HIP(hipGetLastError());
+  }
   return PSKV_OK;
 }

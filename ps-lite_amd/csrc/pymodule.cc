@@ -23,7 +23,7 @@ PyObject* g_tensor_type = nullptr;
 PyObject *g_int64 = nullptr, *g_uint64 = nullptr, *g_float32 = nullptr, *g_int32 = nullptr;
 PyObject* g_raw_stream = nullptr;  // callable: device index -> hipStream_t of torch's current stream, as an int
 PyObject *g_float16 = nullptr, *g_bfloat16 = nullptr;
-PyObject *s_dtype, *s_is_cuda, *s_is_contiguous, *s_numel, *s_data_ptr, *s_shape, *s_stride, *s_get_device;
+PyObject *s_dtype, *s_is_cuda, *s_is_contiguous, *s_numel, *s_data_ptr, *s_shape, *s_stride, *s_get_device, *s_nbytes;
 
 enum Kind { kNone = -1, kHost = PSKV_MEM_HOST, kDevice = PSKV_MEM_DEVICE };
 
@@ -374,7 +374,7 @@ PyObject* replay_run(PyObject*, PyObject* at) {
 // --- operators on rows --------------------------------------------------------------------------------------------------------
 // These check their tensors here, once, and refuse what the calls do not take with TypeError or ValueError.
 
-constexpr int kNoType = -1, kInt32 = 100, kInt64 = 101;  // beside PSKV_F32, PSKV_F16, PSKV_BF16
+constexpr int kNoType = -1, kInt32 = 100, kInt64 = 101, kMemory = 102;  // beside PSKV_F32, PSKV_F16, PSKV_BF16
 
 // A tensor on a GPU, as the calls see it.
 struct Tensor {
@@ -435,6 +435,30 @@ struct Tensor {
     }
     return true;
   }
+  // working memory, of any type; n[0]: bytes
+  bool take_memory(PyObject* o) {
+    if (o == Py_None) return true;
+    if (!g_tensor_type || !PyObject_TypeCheck(o, reinterpret_cast<PyTypeObject*>(g_tensor_type)))
+      return fail(PyExc_TypeError, "a torch tensor is expected");
+    PyObject* at = PyObject_CallMethodNoArgs(o, s_get_device);
+    PyObject* is = at ? PyObject_CallMethodNoArgs(o, s_is_contiguous) : nullptr;
+    PyObject* size = is ? PyObject_GetAttr(o, s_nbytes) : nullptr;
+    PyObject* p = size ? PyObject_CallMethodNoArgs(o, s_data_ptr) : nullptr;
+    if (p) {
+      device = (int)PyLong_AsLong(at);
+      n[0] = PyLong_AsLongLong(size);
+      ptr = PyLong_AsVoidPtr(p);
+      type = kMemory;
+    }
+    const bool whole = is == Py_True;
+    Py_XDECREF(at);
+    Py_XDECREF(is);
+    Py_XDECREF(size);
+    Py_XDECREF(p);
+    if (PyErr_Occurred()) return false;
+    if (device < 0) return fail(PyExc_ValueError, "the tensor is not on the GPU");
+    return whole || fail(PyExc_ValueError, "the tensor is not contiguous");
+  }
   bool has_type(int t) const { return type == t || fail(PyExc_TypeError, t == PSKV_F32 ? "float32 is expected" : "int32 is expected"); }
   bool is_rows_type() const {
     return type == PSKV_F32 || type == PSKV_F16 || type == PSKV_BF16 || fail(PyExc_TypeError, "float32, float16 or bfloat16 is expected");
@@ -461,6 +485,22 @@ struct Tensor {
     return (dims == 2 && n[0] == rows && n[1] == k) || fail(PyExc_ValueError, "its shape does not fit the other tensors'");
   }
 };
+
+// A whole number (a numpy one, too). false: a Python error is set.
+bool whole_number(PyObject* o, unsigned long long* to) {
+  PyObject* i = PyNumber_Index(o);
+  if (!i) return false;
+  *to = PyLong_AsUnsignedLongLong(i);
+  Py_DECREF(i);
+  return !PyErr_Occurred();
+}
+bool whole_number(PyObject* o, long long* to) {
+  PyObject* i = PyNumber_Index(o);
+  if (!i) return false;
+  *to = PyLong_AsLongLong(i);
+  Py_DECREF(i);
+  return !PyErr_Occurred();
+}
 
 // All on one device.
 bool together(std::initializer_list<const Tensor*> all, int* device) {
@@ -503,23 +543,13 @@ bool is_weights(const Tensor& w, const Tensor& place) {
   return w.has_type(PSKV_F32) && w.sized(place.n[0], place.n[1]) && w.dense();
 }
 
-// The working memory of a call: a byte count that it still needs, or 0. -1: refused.
-int64_t working_memory(const Tensor& work, size_t room) {
-  if (!work.given()) return (int64_t)room;
-  if (!work.dense()) return -1;
-  return 0;
-}
-size_t work_bytes(const Tensor& work) {
-  return (size_t)work.count() * (work.type == kInt64 ? 8 : work.type == kInt32 || work.type == PSKV_F32 ? 4 : 2);
-}
-
 // route_sort(experts, E, order, place, offsets, work, stream): a status, or how many bytes of working memory are missing
 PyObject* route_sort(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NEED(want(n, 7));
   Tensor experts("experts"), order("order"), place("place"), offsets("offsets"), work("work");
-  const size_t E = PyLong_AsSize_t(a[1]);
-  NEED(!PyErr_Occurred());
-  NEED(experts.take(a[0]) && order.take(a[2]) && place.take(a[3]) && offsets.take(a[4]) && work.take(a[5], true));
+  unsigned long long E;
+  NEED(whole_number(a[1], &E));
+  NEED(experts.take(a[0]) && order.take(a[2]) && place.take(a[3]) && offsets.take(a[4]) && work.take_memory(a[5]));
   if (experts.type != kInt32 && experts.type != kInt64) NEED(experts.fail(PyExc_TypeError, "int32 or int64 is expected"));
   NEED(experts.dense() && order.has_type(kInt32) && order.dense() && place.has_type(kInt32) && place.dense() &&
        offsets.has_type(kInt32) && offsets.dense());
@@ -530,14 +560,13 @@ PyObject* route_sort(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int device;
   void* stream;
   NEED(together({&experts, &order, &place, &offsets, &work}, &device) && stream_of(a[6], device, &stream));
-  const int64_t missing = working_memory(work, pskv_route_room((size_t)count, E));
-  NEED(missing >= 0);
-  if (missing) return PyLong_FromLongLong(missing);
+  const size_t room = work.given() ? 0 : pskv_route_room((size_t)count, E);
+  if (room) return PyLong_FromSize_t(room);
   int rc;
   Py_BEGIN_ALLOW_THREADS;
   rc = pskv_route_sort(device, stream, experts.ptr, experts.type == kInt64 ? 64 : 32, (size_t)count, E,
                        static_cast<int32_t*>(order.ptr), static_cast<int32_t*>(place.ptr), static_cast<int32_t*>(offsets.ptr),
-                       work.ptr, work_bytes(work));
+                       work.ptr, work.given() ? (size_t)work.n[0] : 0);
   Py_END_ALLOW_THREADS;
   return PyLong_FromLong(rc);
 }
@@ -623,11 +652,10 @@ bool is_positions(const Tensor& at, size_t batch) {
 PyObject* relbias(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NEED(want(n, 9));
   Tensor table("table"), out("out"), scores("scores"), at("q_at");
-  const uint64_t far = PyLong_AsUnsignedLongLong(a[2]);
-  NEED(!PyErr_Occurred());
+  unsigned long long far;
+  long long q_first, k_first;
   const int two_sided = PyObject_IsTrue(a[3]);
-  const long long q_first = PyLong_AsLongLong(a[5]), k_first = PyLong_AsLongLong(a[6]);
-  NEED(!PyErr_Occurred());
+  NEED(two_sided >= 0 && whole_number(a[2], &far) && whole_number(a[5], &q_first) && whole_number(a[6], &k_first));
   NEED(table.take(a[0]) && out.take(a[1]) && scores.take(a[4], true) && at.take(a[7], true) && table.has_type(PSKV_F32) &&
        table.dense() && out.is_rows_type());
   if (table.dims != 2) NEED(table.fail(PyExc_ValueError, "[buckets, heads] is expected"));
@@ -654,12 +682,11 @@ PyObject* relbias(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* relbias_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   NEED(want(n, 9));
   Tensor grad("grad"), grad_table("grad_table"), at("q_at"), work("work");
-  const uint64_t far = PyLong_AsUnsignedLongLong(a[2]);
-  NEED(!PyErr_Occurred());
+  unsigned long long far;
+  long long q_first, k_first;
   const int two_sided = PyObject_IsTrue(a[3]);
-  const long long q_first = PyLong_AsLongLong(a[4]), k_first = PyLong_AsLongLong(a[5]);
-  NEED(!PyErr_Occurred());
-  NEED(grad.take(a[0]) && grad_table.take(a[1]) && at.take(a[6], true) && work.take(a[7], true) && grad.is_rows_type() &&
+  NEED(two_sided >= 0 && whole_number(a[2], &far) && whole_number(a[4], &q_first) && whole_number(a[5], &k_first));
+  NEED(grad.take(a[0]) && grad_table.take(a[1]) && at.take(a[6], true) && work.take_memory(a[7]) && grad.is_rows_type() &&
        grad_table.has_type(PSKV_F32) && grad_table.dense());
   Scores g;
   NEED(g.parse(grad) && is_positions(at, g.n[0]));
@@ -669,14 +696,12 @@ PyObject* relbias_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream;
   NEED(together({&grad, &grad_table, &at, &work}, &device) && stream_of(a[8], device, &stream));
   const size_t buckets = (size_t)grad_table.n[0];
-  const int64_t missing =
-      working_memory(work, pskv_relbias_grad_room(buckets, g.n[1], g.n[0], g.n[2], g.n[3], at.given() ? 1 : 0));
-  NEED(missing >= 0);
-  if (missing) return PyLong_FromLongLong(missing);
+  const size_t room = work.given() ? 0 : pskv_relbias_grad_room(buckets, g.n[1], g.n[0], g.n[2], g.n[3], at.given() ? 1 : 0);
+  if (room) return PyLong_FromSize_t(room);
   Py_BEGIN_ALLOW_THREADS;
   rc = pskv_relbias_grad(device, stream, grad.type, grad.ptr, g.by, buckets, g.n[1], far, two_sided, q_first, k_first,
                          static_cast<int64_t*>(at.ptr), g.n[0], g.n[2], g.n[3], static_cast<float*>(grad_table.ptr), work.ptr,
-                         work_bytes(work));
+                         work.given() ? (size_t)work.n[0] : 0);
   Py_END_ALLOW_THREADS;
   return PyLong_FromLong(rc);
 }
@@ -687,10 +712,8 @@ PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Tensor x("x"), out("out"), step("step"), keys("keys");
   const double p = PyFloat_AsDouble(a[2]);
   NEED(!PyErr_Occurred());
-  const uint64_t seed = PyLong_AsUnsignedLongLong(a[3]);
-  NEED(!PyErr_Occurred());
-  const uint64_t first = PyLong_AsUnsignedLongLong(a[6]);
-  NEED(!PyErr_Occurred());
+  unsigned long long seed, first;
+  NEED(whole_number(a[3], &seed) && whole_number(a[6], &first));
   NEED(x.take(a[0]) && out.take(a[1]) && step.take(a[4], true) && keys.take(a[5], true) && x.is_rows_type() && x.is_matrix() &&
        out.like(x) && out.is_matrix() && out.sized(x.n[0], x.n[1]));
   if (step.given() && (step.type != kInt64 || step.count() != 1)) NEED(step.fail(PyExc_TypeError, "one word of 64 bits is expected"));
@@ -741,6 +764,8 @@ PyMODINIT_FUNC PyInit__native(void) {
   s_shape = PyUnicode_InternFromString("shape");
   s_stride = PyUnicode_InternFromString("stride");
   s_get_device = PyUnicode_InternFromString("get_device");
-  if (!s_dtype || !s_is_cuda || !s_is_contiguous || !s_numel || !s_data_ptr || !s_shape || !s_stride || !s_get_device) return nullptr;
+  s_nbytes = PyUnicode_InternFromString("nbytes");
+  if (!s_dtype || !s_is_cuda || !s_is_contiguous || !s_numel || !s_data_ptr || !s_shape || !s_stride || !s_get_device || !s_nbytes)
+    return nullptr;
   return PyModule_Create(&module);
 }

@@ -540,12 +540,15 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
     s.out[i] = (uint64_t)out_stride[i];
     s.in[i] = scores ? (uint64_t)scores_stride[i] : 0;
   }
+  const uint64_t out_bytes = extent(out_stride, s, type_bytes(type));
+  if (overlap(table, buckets * H * sizeof(float), out, out_bytes) || (q_at && overlap(q_at, B * sizeof(int64_t), out, out_bytes)))
+    return set_error(PSKV_EINVAL, "out overlaps the table or the positions");
   if (scores) {
     const uint64_t a = reinterpret_cast<uintptr_t>(scores), o = reinterpret_cast<uintptr_t>(out), size = type_bytes(type);
     bool same = a == o;
     const size_t n[3] = {B, H, Q};
     for (int i = 0; i < 3; ++i) same = same && (n[i] < 2 || s.in[i] == s.out[i]);
-    if (!same && a < o + extent(out_stride, s, size) && o < a + extent(scores_stride, s, size))
+    if (!same && a < o + out_bytes && o < a + extent(scores_stride, s, size))
       return set_error(PSKV_EINVAL, "out lies in the scores and is not the same tensor");
   }
   const Cut cut = cut_for_bias(B, H, Q, K, type_bytes(type));
@@ -599,6 +602,9 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
     if (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3))
       return set_error(PSKV_EINVAL, "this gradient takes %zu bytes of working memory, %zu given", room, work ? work_bytes : (size_t)0);
   }
+  if (any && (overlap(work, groups * buckets * H * sizeof(float), grad_table, buckets * H * sizeof(float)) ||
+              overlap(work, groups * buckets * H * sizeof(float), grad, extent(grad_stride, s, type_bytes(type)))))
+    return set_error(PSKV_EINVAL, "the working memory overlaps the gradients");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -432,6 +432,14 @@ extern "C" int pskv_route_sort(int device, void* stream, const void* experts, in
   if (room && (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3)))
     return set_error(PSKV_EINVAL, "a sort of %zu choices takes %zu bytes of working memory, %zu given", n, room,
                      work ? work_bytes : (size_t)0);
+  const struct {
+    const void* at;
+    uint64_t bytes;
+  } used[5] = {{experts, n * (uint64_t)index_bits / 8}, {order, n * 4}, {place, n * 4}, {offsets, (E + 1) * 4}, {work, room}};
+  for (int i = 0; i < 5; ++i)
+    for (int j = i + 1; j < 5; ++j)
+      if (overlap(used[i].at, used[i].bytes, used[j].at, used[j].bytes))
+        return set_error(PSKV_EINVAL, "the experts, the answers and the working memory overlap");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -523,6 +531,8 @@ extern "C" int pskv_route_sum_grad(int device, void* stream, int type, const voi
     return set_error(PSKV_EINVAL, "null buffer");
   const size_t size = type_bytes(type);
   const RowSpan to{grad_rows, n_rows, k, grad_rows_stride, size};
+  if (overlap(weights, tokens * choices * 4, grad_weights, tokens * choices * 4))
+    return set_error(PSKV_EINVAL, "the weights and their gradients overlap");
   if (rows_overlap({grad, tokens, k, grad_stride, size}, to) || rows_overlap({rows, n_rows, k, rows_stride, size}, to))
     return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
   DeviceGuard guard(device);

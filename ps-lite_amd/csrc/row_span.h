@@ -25,6 +25,11 @@ inline bool rows_overlap(const RowSpan& a, const RowSpan& b) {
   return in < a.k * a.size || in + b.k * b.size > s;
 }
 
+// Whether two stretches of memory share a byte.
+inline bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  return rows_overlap({a, 1, a_bytes, 0, 1}, {b, 1, b_bytes, 0, 1});
+}
+
 // How many lanes serve a row of `vectors` vectors: a power of two, at most `most`.
 inline unsigned lanes_for(uint64_t vectors, unsigned most) {
   unsigned lanes = 1;

@@ -25,12 +25,13 @@ def _native():
 
 
 def _room(nbytes, like, stream):
-    """Working memory of a call that was not given any, kept from reuse until `stream` has run the call."""
+    """Working memory of a call that was not given any. It belongs to the stream that the call runs on: it may have been used
+    there before, and is used again there behind the call at the earliest."""
     import torch
-    work = torch.empty(-(-nbytes // 4), dtype=torch.int32, device=like.device)
-    if stream is not None:
-        work.record_stream(torch.cuda.ExternalStream(stream, device=like.device))
-    return work
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=like.device)):
+        return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 
 def route_room(n, num_experts):

@@ -301,6 +301,8 @@ BIAS = [  # B, H, Q, K, buckets, far, two_sided, q_first, k_first, own positions
     (1, 1, 9, 9, 32, 128, False, -(1 << 60), 1 << 60, False),
     (2, 2, 513, 511, 128, 1000, True, 0, 0, False),
     (70, 1000, 1, 3, 4, 5, True, 0, 0, False),
+    (64, 13, 1, 5000, 32, 128, False, 0, 0, True),
+    (3, 2, 8, 513, 32, 128, True, 0, 0, True),
 ]
 
 
@@ -391,6 +393,42 @@ def test_gradient_of_bias_against_differences(ops, dev):
         # table + step is off by F of itself, at each of Q * K * H places at most
         slack = float(c.abs().double().sum()) * 2 * F * (float(table.abs().max()) + 0.5) / 0.5 + Q * K * F * float(c.abs().sum())
         assert abs(float(got - grad[u].double().sum())) <= slack
+
+
+@pytest.mark.parametrize("type,B,H,Q,K", [("bfloat16", 2, 64, 1021, 2100), ("float32", 3, 30, 700, 1000), ("float16", 9, 16, 300, 520)])
+def test_gradient_of_many_rows(ops, dev, type, B, H, Q, K):
+    """Sizes at which a wavefront takes 128 rows, or several batches."""
+    import torch
+    announce("relbias_grad, large", type, B, H, Q, K)
+    grad = normal(seeded(3), B, H, Q, K, type=type)
+    got = torch.empty(32, H, device=dev)
+    ops.relbias_grad(grad, got, 128)
+    far = max(Q, K)
+    bucket = torch.tensor([plain_bucket(r, 32, 128, True) for r in range(-far, far + 1)], device=dev)
+    at = bucket[torch.arange(K, device=dev)[None, :] - torch.arange(Q, device=dev)[:, None] + far]
+    total, size = grad.sum(0, dtype=torch.float64), grad.abs().sum(0, dtype=torch.float64)
+    for u in range(32):
+        here = at == u
+        near(got[u], torch.where(here, total, 0.0).sum((1, 2)), (1024 + B) * F * torch.where(here, size, 0.0).sum((1, 2)), "bucket %d" % u)
+
+
+@pytest.mark.parametrize("type", TYPES)
+def test_infinities_stay_in_their_bucket(ops, dev, type):
+    import torch
+    announce("relbias_grad, special values", type)
+    H, Q, K = 3, 70, 613
+    grad = normal(seeded(4), 2, H, Q, K, type=type)
+    clean = torch.empty(32, H, device=dev)
+    ops.relbias_grad(grad, clean, 128)
+    want = clean.clone()
+    for h, i, j, value in [(0, 5, 5, float("inf")), (1, 69, 612, float("nan")), (2, 69, 0, float("-inf")), (2, 0, 3, float("inf")),
+                           (0, 33, 610, float("nan"))]:
+        grad[1, h, i, j] = value
+        u = plain_bucket(j - i, 32, 128, True)
+        want[u, h] = float("nan") if not np.isinf(value) or not torch.isfinite(want[u, h]) else value
+    got = torch.empty(32, H, device=dev)
+    ops.relbias_grad(grad, got, 128)
+    assert torch.equal(torch.nan_to_num(got, nan=1e30), torch.nan_to_num(want, nan=1e30))
 
 
 def test_bias_without_batch_and_empty(ops, dev):
@@ -551,6 +589,127 @@ def test_shapes_and_types_are_refused(ops, capi, dev):
     ops.dropout(wide[:, :8], wide[:, 8:], 0.5, 1)  # columns beside each other are fine
     ops.route_rows(x[:1].expand(4, 8), place[:, :1].contiguous(), rows)  # so is one row read four times
     torch.cuda.synchronize()
+
+
+def test_numbers_and_working_memory_of_other_types(ops, dev):
+    import torch
+    announce("ops, numpy numbers, bytes as working memory")
+    experts = torch.randint(0, 9, (5000, 1), device=dev)
+    work = torch.empty(ops.route_room(5000, 9), dtype=torch.uint8, device=dev)
+    a, b = sort(ops, experts, 9), sort(ops, experts, np.int64(9), work=work)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    x = torch.ones(4, 9, device=dev)
+    y, z = torch.empty_like(x), torch.empty_like(x)
+    ops.dropout(x, y, 0.5, 77)
+    ops.dropout(x, z, np.float64(0.5), np.uint64(77))
+    assert torch.equal(y, z)
+    with pytest.raises(ValueError):
+        ops.route_sort(experts, 9, a[0], a[1], a[2], work=work[::2])
+    with pytest.raises(ValueError):
+        ops.route_sort(experts, 9, a[0], a[1], a[2], work=work.cpu())
+
+
+def test_many_choices(ops, dev):
+    import torch
+    announce("route_sort, 20,000,001 choices")
+    g = seeded(8)
+    experts = torch.randint(-1, 300, (20000001, 1), generator=g, device=dev, dtype=torch.int32)
+    order, place, offsets = sort(ops, experts, 300)
+    key = torch.where(experts.view(-1) < 0, 300, experts.view(-1))
+    held = torch.sort(key, stable=True)
+    n = int((held.values < 300).sum())
+    assert torch.equal(order[:n], held.indices[:n].to(torch.int32)) and bool((order[n:] == -1).all())
+    assert torch.equal(offsets, torch.searchsorted(held.values, torch.arange(301, device=dev, dtype=torch.int32)).to(torch.int32))
+    assert torch.equal(place.view(-1)[held.indices[:n]], torch.arange(n, device=dev, dtype=torch.int32))
+    assert bool((place.view(-1)[held.indices[n:]] == -1).all())
+
+
+def test_rows_beyond_32_bits(ops, dev):
+    """Rows that lie 2^32 elements and more into their memory."""
+    import torch
+    announce("route, 70,001 rows of 65,536")
+    R, k = 70001, 65536
+    g = seeded(6)
+    rows = torch.zeros(R, k, dtype=torch.bfloat16, device=dev)
+    x, grad = normal(g, 3, k, type="bfloat16"), normal(g, 3, k, type="bfloat16")
+    place = torch.tensor([[0, R - 1], [65537, -1], [R - 2, 32769]], dtype=torch.int32, device=dev)
+    ops.route_rows(x, place, rows)
+    named = torch.tensor([0, R - 1, 65537, R - 2, 32769], device=dev)
+    assert torch.equal(rows[named], x[torch.tensor([0, 0, 1, 2, 2], device=dev)])
+    rows[named] = 0
+    assert not bool(rows.view(torch.int32).any())
+    answers = normal(g, 5, k, type="bfloat16")
+    rows[named] = answers
+    out = torch.empty_like(x)
+    ops.route_sum(rows, place, out)
+    want = torch.stack([answers[0].double() + answers[1].double(), answers[2].double(), answers[3].double() + answers[4].double()])
+    near(out, want, rounded(want, 2 * F * want.abs(), "bfloat16"), "sum")
+    weights, grad_weights = torch.ones(3, 2, device=dev), torch.empty(3, 2, device=dev)
+    grad_rows = torch.zeros_like(rows)
+    ops.route_sum_grad(grad, rows, place, weights, grad_rows, grad_weights)
+    assert torch.equal(grad_rows[named], grad[torch.tensor([0, 0, 1, 2, 2], device=dev)])
+    grad_rows[named] = 0
+    assert not bool(grad_rows.view(torch.int32).any())
+
+
+def test_scores_beyond_32_bits(ops, dev):
+    import torch
+    announce("relbias, a batch 2^31 elements apart")
+    B, H, Q, K, apart = 3, 2, 9, 601, (1 << 31) + 24
+    whole = torch.zeros((B - 1) * apart + H * Q * K, dtype=torch.bfloat16, device=dev)
+    out = whole.as_strided((B, H, Q, K), (apart, Q * K, K, 1))
+    g = seeded(7)
+    table, scores = normal(g, 32, H), normal(g, B, H, Q, K, type="bfloat16")
+    plain, sums, more = torch.empty_like(scores), torch.empty_like(table), torch.empty_like(table)
+    ops.relbias(table, plain, 128, scores=scores)
+    ops.relbias(table, out, 128, scores=scores)
+    assert torch.equal(out, plain)
+    ops.relbias(table, out, 128, scores=out)
+    ops.relbias(table, plain, 128, scores=plain)
+    assert torch.equal(out, plain)
+    ops.relbias_grad(out, sums, 128)
+    ops.relbias_grad(plain, more, 128)
+    assert torch.equal(sums, more)
+
+
+@pytest.mark.parametrize("type", ["bfloat16", "float32"])
+def test_dropout_in_pieces(ops, dev, type):
+    """More rows than one launch counts."""
+    import torch
+    announce("dropout, 2^31 + 1000 rows", type)
+    n = (1 << 31) + 1000
+    x = torch.full((1, 1), 2.0, device=dev).to(getattr(torch, type)).expand(n, 1)
+    out = torch.empty(n, 1, dtype=getattr(torch, type), device=dev)
+    ops.dropout(x, out, 0.5, 1234, first=5)
+    for at in (0, (1 << 31) - 600, (1 << 31) - 512, (1 << 31) - 300, (1 << 31) - 10, n - 100):
+        keep = plain_bits(np.arange(at + 5, at + 105, dtype=np.uint64), 1, 1234) >= 32768
+        assert np.array_equal(out[at:at + 100].float().cpu().numpy(), np.where(keep, 4.0, 0.0)), at
+
+
+def test_two_threads(ops, capi, dev):
+    """Calls share no state: two threads, each on a stream of its own."""
+    import threading
+    import torch
+    announce("ops, two threads")
+    plain = chain_state(ops, capi, dev, 3)
+    chain(ops, plain)
+    states, sides = [chain_state(ops, capi, dev, 3) for _ in range(2)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def work(s, side):
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                chain(ops, s)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(states, sides)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for s in states:
+        for name in ANSWERS:
+            assert torch.equal(s[name], plain[name]), name
 
 
 def chain(ops, s):

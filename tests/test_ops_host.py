@@ -119,7 +119,9 @@ SORT = dict(bits=64, n=100, E=8, experts=AT[0], order=AT[1], place=AT[2], offset
 
 @pytest.mark.parametrize("change", [dict(bits=16), dict(E=0), dict(E=2049), dict(n=1 << 31), dict(experts=None), dict(order=None),
                                     dict(place=None), dict(offsets=None), dict(n=10000), dict(n=10000, work=AT[4], room=8),
-                                    dict(n=10000, work=ctypes.c_void_p((1 << 40) + 2), room=1 << 20)])
+                                    dict(n=10000, work=ctypes.c_void_p((1 << 40) + 2), room=1 << 20), dict(order=AT[0]),
+                                    dict(place=ctypes.c_void_p(AT[0].value + 796)), dict(place=AT[1]), dict(offsets=AT[2]),
+                                    dict(n=10000, work=AT[3], room=1 << 20)])
 def test_sort_refuses(capi, change):
     a = dict(SORT, **change)
     assert capi.load().pskv_route_sort(0, None, a["experts"], a["bits"], a["n"], a["E"], a["order"], a["place"], a["offsets"],
@@ -164,7 +166,7 @@ def test_rows_refuse(capi, which, change):
     ("rows", dict(rows=None)), ("rows", dict(rows_stride=15)), ("rows", dict(rows=AT[0])),
     ("rows", dict(rows=ctypes.c_void_p(AT[0].value + 10 * 64 - 4))), ("sum", dict(rows=None)), ("sum", dict(x_stride=15)),
     ("sum", dict(x=AT[2])), ("grad", dict(weights=None)), ("grad", dict(grad_weights=None)), ("grad", dict(grad_rows=None)),
-    ("grad", dict(grad_stride=15)), ("grad", dict(grad_rows=AT[0])), ("grad", dict(grad_rows=AT[2]))])
+    ("grad", dict(grad_weights=AT[3])), ("grad", dict(grad_stride=15)), ("grad", dict(grad_rows=AT[0])), ("grad", dict(grad_rows=AT[2]))])
 def test_rows_refuse_what_they_write(capi, which, change):
     assert _rows_call(capi, which, dict(ROWS, **change)) == capi.EINVAL
 
@@ -196,7 +198,7 @@ def test_bias_refuses(capi, grad, change):
 
 
 @pytest.mark.parametrize("grad,change", [
-    (False, dict(table=None)), (False, dict(out=None)), (False, dict(out_by=None)), (False, dict(out_by=_strides(0, 100, 10))),
+    (False, dict(table=None)), (False, dict(out=AT[0])), (False, dict(out=None)), (True, dict(work=AT[3])), (True, dict(work=AT[1])), (False, dict(out_by=None)), (False, dict(out_by=_strides(0, 100, 10))),
     (False, dict(out_by=_strides(400, 100, 9))), (False, dict(out_by=_strides(400, 99, 10))), (False, dict(out_by=_strides(400, 100, 0))),
     (False, dict(out=ctypes.c_void_p(AT[1].value + 4))), (False, dict(out=AT[1], in_by=_strides(0, 100, 10))),
     (True, dict(scores=None)), (True, dict(grad_table=None)), (True, dict(work=None)), (True, dict(room=100)),
