@@ -190,10 +190,15 @@ def _prepare_dropout(case, g):
 
 # --- one pass ----------------------------------------------------------------------------------------------------
 
+_ops = None
+
+
 def run(state):
+    global _ops
     if own:
-        ops = importlib.import_module("ps-lite_amd").ops
-        return globals()["_own_" + state["case"]["kind"]](state, ops)
+        if _ops is None:  # (a program imports the package once, not with every call)
+            _ops = importlib.import_module("ps-lite_amd").ops
+        return globals()["_own_" + state["case"]["kind"]](state, _ops)
     return globals()["_plain_" + state["case"]["kind"]](state)
 
 
