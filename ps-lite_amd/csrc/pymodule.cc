@@ -401,10 +401,7 @@ struct Tensor {
     device = (int)PyLong_AsLong(at);
     Py_DECREF(at);
     if (PyErr_Occurred()) return false;
-    PyObject* cuda = PyObject_GetAttr(o, s_is_cuda);
-    if (!cuda) return false;
-    Py_DECREF(cuda);
-    if (cuda != Py_True) return fail(PyExc_ValueError, "the tensor is not on the GPU");
+    if (device < 0) return fail(PyExc_ValueError, "the tensor is not on the GPU");
     PyObject* d = PyObject_GetAttr(o, s_dtype);
     if (!d) return false;
     Py_DECREF(d);

@@ -8,6 +8,7 @@
 #include <new>
 
 #include "host_common.h"
+#include "lanes.h"
 #include "relbias.h"
 #include "row_types.h"
 
@@ -112,37 +113,6 @@ __device__ __forceinline__ void store_some(T* p, const float (&y)[N], unsigned n
   const T a = done ? e[N - 4] : e[0], b = done ? e[N - 3] : e[1], c = done ? e[N - 2] : e[2];
   if (n & 2) *reinterpret_cast<Two*>(p + done) = Two{a, b};
   if (n & 1) p[done + (n & 2)] = n & 2 ? c : a;
-}
-
-// The lane below's `v`; lane 0 gets `first`.
-__device__ __forceinline__ float from_below(float v, float first) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, first), __builtin_bit_cast(int, v),
-                                                               0x138 /* wave_shr:1 */, 0xf, 0xf, false));
-}
-
-// What the lane that CONTROL names has, 0 where there is none or the lane's row of 16 is not in ROWS.
-template <int CONTROL, int ROWS>
-__device__ __forceinline__ uint32_t dpp(uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, ROWS, 0xf, false);
-}
-
-// One step of a sum along the lanes that starts anew where `starts` is set: what has been summed up to the lane that CONTROL names
-// comes in, unless a start lies between.
-template <int CONTROL, int ROWS>
-__device__ __forceinline__ void sum_step(float& sum, uint32_t& starts) {
-  const float up = __builtin_bit_cast(float, dpp<CONTROL, ROWS>(__builtin_bit_cast(uint32_t, sum)));
-  const uint32_t there = dpp<CONTROL, ROWS>(starts);
-  sum = starts ? sum : sum + up;
-  starts |= there;
-}
-__device__ __forceinline__ float sum_along(float sum, uint32_t starts) {
-  sum_step<0x111 /* row_shr:1 */, 0xf>(sum, starts);
-  sum_step<0x112, 0xf>(sum, starts);
-  sum_step<0x114, 0xf>(sum, starts);
-  sum_step<0x118, 0xf>(sum, starts);
-  sum_step<0x142 /* row_bcast:15 */, 0xa>(sum, starts);
-  sum_step<0x143 /* row_bcast:31 */, 0xc>(sum, starts);
-  return sum;
 }
 
 // A lane's part of the rows of a tile: columns c to c + N - 1, or what there is of them.
