@@ -38,7 +38,8 @@ struct Divisor {
   }
 };
 
-// 16-bit types: a lane takes the 8 columns of a draw, 16 bytes. Indexes are those of draws.
+// 16-bit types: a lane takes the 8 columns of a draw, 16 bytes. Indexes are those of draws. The ten rounds' products (16 cycles each)
+// and the memory take about the same time: 65,536 rows of 2,048 bf16 in 90 us, 6.0 TB/s; 4,099 of 1,001 in 5.5.
 template <typename T, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_dropout(const T* x, T* out, const uint64_t* __restrict__ keys, uint64_t first,
                                                      const uint64_t* __restrict__ step, uint64_t seed, uint32_t draws, uint32_t k,
@@ -75,7 +76,8 @@ __device__ __forceinline__ uint32_t of_neighbour(uint32_t v) {  // lanes 2i and 
 
 // float32: a draw's 8 columns are 32 bytes, and lanes that each take 32 bytes leave every access half of its lines. So a lane
 // takes four columns here and four 64 lanes further on; of two neighbours the even one draws for both here, the odd one there,
-// and they exchange halves. Indexes are those of quads of columns, two to a draw.
+// and they exchange halves. Indexes are those of quads of columns, two to a draw. 1M rows of 64: 80 us, 6.5 TB/s, past the caches
+// (32 bytes to a lane: 100, and 237 past the caches; every lane drawing for its four columns: 109).
 template <bool PAST>
 __global__ __launch_bounds__(kBlock) void k_dropout_pairs(const float* x, float* out, const uint64_t* __restrict__ keys, uint64_t first,
                                                            const uint64_t* __restrict__ step, uint64_t seed, uint32_t quads, uint32_t k,

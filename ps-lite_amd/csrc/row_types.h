@@ -56,7 +56,7 @@ inline void with_flag(bool flag, F f) {
     f(std::false_type());
 }
 
-// What moves more than so many bytes does not stay in the memory-side cache anyway.
+// What moves more than so many bytes, the size of the memory-side cache, does not stay there anyway.
 constexpr uint64_t kPastBytes = 256u << 20;
 
 }  // namespace pskv
