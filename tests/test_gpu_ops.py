@@ -237,6 +237,28 @@ def test_gradients_against_differences(ops, dev):
             + 2 * F * (k + 1) * T * K * k * float(c.abs().max() * (rows.abs().max() + weights.abs().max()))
 
 
+def test_no_tokens_and_no_rows(ops, dev):
+    import torch
+    announce("route, nothing there")
+    i32 = dict(dtype=torch.int32, device=dev)
+    rows = torch.full((4, 6), 7.0, device=dev)
+    empty, none = torch.empty(0, 6, device=dev), torch.empty(0, 2, **i32)
+    ops.route_rows(empty, none, rows)
+    ops.route_sum(rows, none, empty, weights=torch.empty(0, 2, device=dev))
+    ops.route_sum_grad(empty, rows, none, torch.empty(0, 2, device=dev), rows.clone(), torch.empty(0, 2, device=dev))
+    assert bool((rows == 7).all())
+    # tokens without any row: nothing is here
+    x, place = torch.ones(3, 6, device=dev), torch.tensor([[0, 1], [-1, 5], [0, 0]], **i32)
+    weights, grad_weights = torch.full((3, 2), float("nan"), device=dev), torch.full((3, 2), 7.0, device=dev)
+    out = torch.full((3, 6), 7.0, device=dev)
+    ops.route_rows(x, place, empty)
+    ops.route_sum(empty, place, out, weights=weights)
+    ops.route_sum_grad(x, empty, place, weights, torch.empty_like(empty), grad_weights)
+    assert bool((out == 0).all()) and bool((grad_weights == 0).all())
+    y = torch.empty(0, 6, device=dev)
+    ops.dropout(y, y, 0.5, 1)
+
+
 def test_choices_of_one_expert_twice(ops, dev):
     """A token may name an expert twice: it has two rows there. Its row's gradient takes both."""
     import torch
