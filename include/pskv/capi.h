@@ -355,8 +355,8 @@ int pskv_relbias(int device, void* stream, int type, const float* table, size_t 
 /* The bucket of one relative position (host), or a negative PSKV_E* code. */
 int pskv_relbias_bucket(int64_t rel, size_t buckets, uint64_t max_distance, int two_sided);
 /* Its gradient: grad_table[u * H + h] = the sum of grad[b,h,i,j] over what bucket u was added to; 0 for a bucket that is not
- * used: the values of a push to the table of the biases. `work`: pskv_relbias_grad_room(...) bytes, aligned to 4 (own_positions:
- * whether q_at is given). */
+ * used: the values of a push to the table of the biases. `work`: pskv_relbias_grad_room(...) bytes, aligned to 4, none (NULL)
+ * where that is 0 (own_positions: whether q_at is given). */
 size_t pskv_relbias_grad_room(size_t buckets, size_t H, size_t B, size_t Q, size_t K, int own_positions);
 int pskv_relbias_grad(int device, void* stream, int type, const void* grad, const int64_t* grad_stride, size_t buckets, size_t H,
                       uint64_t max_distance, int two_sided, int64_t q_first, int64_t k_first, const int64_t* q_at, size_t B,

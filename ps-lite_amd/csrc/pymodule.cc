@@ -540,9 +540,28 @@ bool is_weights(const Tensor& w, const Tensor& place) {
   return w.has_type(PSKV_F32) && w.sized(place.n[0], place.n[1]) && w.dense();
 }
 
-// route_sort(experts, E, order, place, offsets, work, stream): a status, or how many bytes of working memory are missing
+// Working memory of a call that was not given any, from allocate(bytes, a tensor of the call, stream); kept until the call has been
+// enqueued.
+class Room {
+ public:
+  ~Room() { Py_XDECREF(held_); }
+  bool take(Tensor& work, size_t bytes, PyObject* allocate, PyObject* like, PyObject* stream) {
+    if (work.given() || bytes == 0) return true;
+    PyObject* size = PyLong_FromSize_t(bytes);
+    if (!size) return false;
+    PyObject* args[] = {size, like, stream};
+    held_ = PyObject_Vectorcall(allocate, args, 3, nullptr);
+    Py_DECREF(size);
+    return held_ && work.take_memory(held_);
+  }
+
+ private:
+  PyObject* held_ = nullptr;
+};
+
+// route_sort(experts, E, order, place, offsets, work, stream, allocate)
 PyObject* route_sort(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  NEED(want(n, 7));
+  NEED(want(n, 8));
   Tensor experts("experts"), order("order"), place("place"), offsets("offsets"), work("work");
   unsigned long long E;
   NEED(whole_number(a[1], &E));
@@ -557,8 +576,8 @@ PyObject* route_sort(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int device;
   void* stream;
   NEED(together({&experts, &order, &place, &offsets, &work}, &device) && stream_of(a[6], device, &stream));
-  const size_t room = work.given() ? 0 : pskv_route_room((size_t)count, E);
-  if (room) return PyLong_FromSize_t(room);
+  Room room;
+  NEED(room.take(work, pskv_route_room((size_t)count, E), a[7], a[0], a[6]));
   int rc;
   Py_BEGIN_ALLOW_THREADS;
   rc = pskv_route_sort(device, stream, experts.ptr, experts.type == kInt64 ? 64 : 32, (size_t)count, E,
@@ -675,9 +694,9 @@ PyObject* relbias(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(rc);
 }
 
-// relbias_grad(grad, grad_table, max_distance, two_sided, q_first, k_first, q_at, work, stream): as route_sort
+// relbias_grad(grad, grad_table, max_distance, two_sided, q_first, k_first, q_at, work, stream, allocate)
 PyObject* relbias_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  NEED(want(n, 9));
+  NEED(want(n, 10));
   Tensor grad("grad"), grad_table("grad_table"), at("q_at"), work("work");
   unsigned long long far;
   long long q_first, k_first;
@@ -693,8 +712,8 @@ PyObject* relbias_grad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream;
   NEED(together({&grad, &grad_table, &at, &work}, &device) && stream_of(a[8], device, &stream));
   const size_t buckets = (size_t)grad_table.n[0];
-  const size_t room = work.given() ? 0 : pskv_relbias_grad_room(buckets, g.n[1], g.n[0], g.n[2], g.n[3], at.given() ? 1 : 0);
-  if (room) return PyLong_FromSize_t(room);
+  Room room;
+  NEED(room.take(work, pskv_relbias_grad_room(buckets, g.n[1], g.n[0], g.n[2], g.n[3], at.given() ? 1 : 0), a[9], a[0], a[8]));
   Py_BEGIN_ALLOW_THREADS;
   rc = pskv_relbias_grad(device, stream, grad.type, grad.ptr, g.by, buckets, g.n[1], far, two_sided, q_first, k_first,
                          static_cast<int64_t*>(at.ptr), g.n[0], g.n[2], g.n[3], static_cast<float*>(grad_table.ptr), work.ptr,

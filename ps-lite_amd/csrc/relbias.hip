@@ -272,21 +272,22 @@ constexpr unsigned kCols = 64 * kWide;  // of a wavefront
 
 // The same the other way round: rows are summed over the batch, then along the diagonals, which move up one lane every
 // eight rows; those that leave lane 63 and those that are there in the end are summed by bucket, 64 neighbouring diagonals
-// at a time. Every sum has one order. partial[head][bucket][workgroup of the head]. 8 x 16 x 1024 x 1024 bf16: 45 us, 6.0 TB/s, and 5 for
+// at a time. Every sum has one order. partial[head][bucket][workgroup of the head], or the gradient itself where a head has one
+// workgroup. 8 x 16 x 1024 x 1024 bf16: 45 us, 6.0 TB/s, and 5 for
 // k_relbias_join (a lane to a diagonal, element by element: 460).
 template <typename T, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ grad, const int64_t* __restrict__ q_at,
-                                                          float* __restrict__ partial, unsigned buckets, unsigned tiles,
-                                                          Cut cut, Shape s, Buckets b) {
+                                                          float* __restrict__ partial, float* __restrict__ grad_table,
+                                                          unsigned buckets, unsigned tiles, Cut cut, Shape s, Buckets b) {
   __shared__ uint32_t border[kMostBuckets / 2 + 1];
   __shared__ float diagonal[kWaves][kMostRows + kCols];
   __shared__ float sums[kWaves][kMostBuckets];
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const uint64_t head = blockIdx.y;
-  const unsigned tile = blockIdx.x * kWaves + wave;
   fetch_borders(border, b);
   for (unsigned u = lane; u < buckets; u += 64) sums[wave][u] = 0.0f;
   __syncthreads();
+  const unsigned tile = blockIdx.x * kWaves + wave;
   if (tile < tiles) {
     const Tile t(tile, cut, s);  // (of any head: cut.parts is 1)
     const Span<kWide> span(t.c0, lane, s.K);
@@ -332,26 +333,26 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // diagonal[x] is the one that is x - reach columns to the right of the tile's corner
     const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0 - reach));
+    // (those that no element of the tile is on are left out)
+    const unsigned reached = reach + (s.K - t.c0 < kCols ? (unsigned)(s.K - t.c0) : kCols);
     // Far from the main diagonal 64 of them have one bucket: those are added up lane by lane until another one comes.
     float run = 0.0f;
-    unsigned of = kMostBuckets;
+    unsigned now = kMostBuckets;
     auto finish = [&] {
-      if (of == kMostBuckets) return;
+      if (now == kMostBuckets) return;
       run = sum_along(run, 0);
-      if (lane == 63) sums[wave][of] += run;
+      if (lane == 63) sums[wave][now] += run;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       run = 0.0f;
-      of = kMostBuckets;
+      now = kMostBuckets;
     };
-    for (unsigned x0 = 0; x0 < reach + kCols; x0 += 64) {
-      const unsigned x = x0 + lane;
-      float sum = x < reach + kCols ? diagonal[wave][x] : 0.0f;
-      const unsigned u = bucket_of(b, border, rel + (int)x), first = __builtin_amdgcn_readfirstlane(u);
+    auto sum_up = [&](unsigned u, float sum) {
+      const unsigned first = __builtin_amdgcn_readfirstlane(u);
       if (__all(u == first)) {
-        if (first != of) finish();
-        of = first;
+        if (first != now) finish();
+        now = first;
         run += sum;
-        continue;
+        return;
       }
       finish();
       // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
@@ -359,6 +360,22 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
       sum = sum_along(sum, lane == 0 || below != u ? 1 : 0);
       if (lane == 63 || above != u) sums[wave][u] += sum;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    const unsigned first = bucket_of(b, border, rel), last = bucket_of(b, border, rel + (int)reached - 1);
+    if (first == last) {  // a tile far from the main diagonal: so have all between
+      now = first;
+      for (unsigned x = lane; x < reached; x += 64) run += diagonal[wave][x];
+    } else {
+      unsigned next_u = bucket_of(b, border, rel + (int)lane);
+      float next = lane < reached ? diagonal[wave][lane] : 0.0f;
+      for (unsigned x = lane; x - lane < reached;) {
+        const unsigned u = next_u;
+        const float part = next;
+        x += 64;  // (looked up while the ones before are summed)
+        next = x < reached ? diagonal[wave][x] : 0.0f;
+        next_u = bucket_of(b, border, rel + (int)x);
+        sum_up(u, part);
+      }
     }
     finish();
   }
@@ -367,7 +384,10 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     float sum = sums[0][u];
 #pragma unroll
     for (unsigned w = 1; w < kWaves; ++w) sum += sums[w][u];
-    partial[(head * buckets + u) * gridDim.x + blockIdx.x] = sum;
+    if (gridDim.x == 1)
+      grad_table[u * s.H + head] = sum;
+    else
+      partial[(head * buckets + u) * gridDim.x + blockIdx.x] = sum;
   }
 }
 
@@ -482,6 +502,7 @@ Cut cut_for_sums(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
   return c;
 }
 
+// The workgroups of a head.
 uint64_t groups_of(const Cut& c) { return (c.tiles() + kWaves - 1) / kWaves; }
 
 }  // namespace
@@ -550,7 +571,8 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
 
 extern "C" size_t pskv_relbias_grad_room(size_t buckets, size_t H, size_t B, size_t Q, size_t K, int own_positions) {
   if (B == 0 || Q == 0 || K == 0 || B > (1u << 20) || Q > (1u << 20) || K > (1u << 30)) return 0;
-  return groups_of(cut_for_sums(B, H, Q, K, own_positions != 0)) * buckets * H * sizeof(float);
+  const uint64_t groups = groups_of(cut_for_sums(B, H, Q, K, own_positions != 0));
+  return groups == 1 ? 0 : groups * buckets * H * sizeof(float);
 }
 
 extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void* grad, const int64_t* grad_stride,
@@ -574,11 +596,13 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
     cut = cut_for_sums(B, H, Q, K, q_at != nullptr);
     groups = groups_of(cut);
     if (groups > kMostTiles / kBlock) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
-    const size_t room = groups * buckets * H * sizeof(float);
-    if (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3))
+    const size_t room = groups == 1 ? 0 : groups * buckets * H * sizeof(float);
+    if (room == 0)
+      work = nullptr;
+    else if (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3))
       return set_error(PSKV_EINVAL, "this gradient takes %zu bytes of working memory, %zu given", room, work ? work_bytes : (size_t)0);
   }
-  if (any && (overlap(work, groups * buckets * H * sizeof(float), grad_table, buckets * H * sizeof(float)) ||
+  if (work && (overlap(work, groups * buckets * H * sizeof(float), grad_table, buckets * H * sizeof(float)) ||
               overlap(work, groups * buckets * H * sizeof(float), grad, extent(grad_stride, s, type_bytes(type)))))
     return set_error(PSKV_EINVAL, "the working memory overlaps the gradients");
   DeviceGuard guard(device);
@@ -591,10 +615,11 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
       // (of several gradients of 83 MB in turn, 31 us each, some is still in the memory-side cache, 34 past it; of 134 MB 32 and 29)
       auto kernel = B * H * Q * K * sizeof(T) > kPastBytes / 2 ? k_relbias_sums<T, true> : k_relbias_sums<T, false>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad),
-                         q_at, partial, (unsigned)buckets, (unsigned)cut.tiles(), cut, s, b);
+                         q_at, partial, grad_table, (unsigned)buckets, (unsigned)cut.tiles(), cut, s, b);
     });
-  hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(64), 0, st, partial, (unsigned)buckets,
-                     (unsigned)groups, (uint64_t)H, grad_table);
+  if (groups != 1)
+    hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(64), 0, st, partial, (unsigned)buckets,
+                       (unsigned)groups, (uint64_t)H, grad_table);
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
 }

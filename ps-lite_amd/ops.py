@@ -44,10 +44,7 @@ def route_sort(experts, num_experts, order, place, offsets, work=None, stream=No
     each choice went, order (int32, as many) the choice at each place, offsets (int32, num_experts + 1) where each expert's
     begin. Numbers outside 0 .. num_experts - 1 are choices that are not here: their place is -1, and order is -1 behind the
     last expert's. work: at least route_room() bytes, for a program that keeps them; else they are allocated."""
-    native = _native()
-    rc = native.route_sort(experts, num_experts, order, place, offsets, work, stream)
-    if rc > 0:
-        rc = native.route_sort(experts, num_experts, order, place, offsets, _room(rc, experts, stream), stream)
+    rc = _native().route_sort(experts, num_experts, order, place, offsets, work, stream, _room)
     if rc:
         _check(rc)
 
@@ -94,14 +91,16 @@ def relbias(table, out, max_distance, two_sided=True, scores=None, q_first=0, k_
         _check(rc)
 
 
+def relbias_grad_room(buckets, batch, heads, queries, keys, own_positions=False):
+    """Bytes of working memory that a gradient of [batch, heads, queries, keys] takes (0: none); own_positions: with q_at."""
+    return capi.load().pskv_relbias_grad_room(buckets, heads, batch, queries, keys, 1 if own_positions else 0)
+
+
 def relbias_grad(grad, grad_table, max_distance, two_sided=True, q_first=0, k_first=0, q_at=None, work=None, stream=None):
     """The gradient of the table: grad_table[u, h] (float32, all of it is written) = the sum of grad over what bucket u was
-    added to, the values of a push to the table of rows."""
-    native = _native()
-    rc = native.relbias_grad(grad, grad_table, max_distance, two_sided, q_first, k_first, q_at, work, stream)
-    if rc > 0:
-        work = _room(rc, grad, stream)
-        rc = native.relbias_grad(grad, grad_table, max_distance, two_sided, q_first, k_first, q_at, work, stream)
+    added to, the values of a push to the table of rows. work: at least relbias_grad_room() bytes, for a program that keeps
+    them; else they are allocated."""
+    rc = _native().relbias_grad(grad, grad_table, max_distance, two_sided, q_first, k_first, q_at, work, stream, _room)
     if rc:
         _check(rc)
 

@@ -597,7 +597,7 @@ def test_shapes_and_types_are_refused(ops, capi, dev):
         (TypeError, lambda: ops.relbias(table, s, 128, q_at=place[:2, 0])), (ValueError, lambda: ops.relbias(table, s, 128, q_at=torch.zeros(3, dtype=torch.int64, device=dev))),
         (capi.PskvError, lambda: ops.relbias(table, s, 8)), (capi.PskvError, lambda: ops.relbias(table, s[:, :1].expand(2, 2, 4, 4), 128)),
         (ValueError, lambda: ops.relbias_grad(s, table[:, :1], 128)), (TypeError, lambda: ops.relbias_grad(s, table.double(), 128)),
-        (capi.PskvError, lambda: ops.relbias_grad(s, table, 128, work=order)),
+        (capi.PskvError, lambda: ops.relbias_grad(torch.zeros(2, 2, 100, 100, device=dev), table, 128, work=order)),
         (ValueError, lambda: ops.dropout(x, rows, 0.5, 1)), (capi.PskvError, lambda: ops.dropout(x, x, 1.5, 1)),
         (ValueError, lambda: ops.dropout(x, x, 0.5, 1, keys=order.long())), (TypeError, lambda: ops.dropout(x, x, 0.5, 1, keys=order[:4])),
         (OverflowError, lambda: ops.dropout(x, x, 0.5, 1 << 64)), (TypeError, lambda: ops.dropout(x, x, 0.5, 1, step=order[:1])),
@@ -757,7 +757,7 @@ def chain_state(ops, capi, dev, seed, type="bfloat16"):
     T, K, k, dt = 6000, 3, 40, getattr(torch, type)
     n = T * K
     i32 = dict(dtype=torch.int32, device=dev)
-    room = capi.load().pskv_relbias_grad_room(32, 3, 2, 20, 300, 1)
+    room = ops.relbias_grad_room(32, 2, 3, 20, 300, own_positions=True)
     return {"experts": torch.randint(-2, 40, (T, K), generator=g, device=dev), "x": normal(g, T, k, type=type),
             "keys": torch.randint(-(1 << 63), (1 << 63) - 1, (T,), generator=g, device=dev), "step": torch.zeros(1, dtype=torch.int64, device=dev),
             "weights": torch.rand(T, K, generator=g, device=dev), "table": normal(g, 32, 3), "scores": normal(g, 2, 3, 20, 300, type=type),
