@@ -19,8 +19,6 @@ namespace {
 
 constexpr unsigned kSortBlock = 1024;
 constexpr unsigned kSortWaves = kSortBlock / 64;
-constexpr unsigned kSortItems = 4;  // choices per lane; one where there are not more of them than lanes
-constexpr unsigned kSortTile = kSortBlock * kSortItems;
 // Up to so many counts, every workgroup adds up the tiles' for itself; beyond, a launch of its own does. Both sides, with the
 // launch's own start of about 1 us: 64 tiles of 257 counts 14.5 and 16.9 us, 128 of 257 19.4 and 18.6, 32 of 1,025 19.0 and 18.3,
 // 512 of 257 61 and 36, 64 of 2,048 32 and 22.
@@ -34,19 +32,19 @@ __device__ __forceinline__ unsigned bin_of(const I* experts, uint64_t i, unsigne
 }
 
 // How many choices of every bin a tile has: counts[tile][bin].
-template <typename I>
+template <typename I, unsigned ITEMS>
 __global__ __launch_bounds__(kSortBlock) void k_route_count(const I* __restrict__ experts, uint64_t n, unsigned E,
                                                              unsigned* __restrict__ counts) {
   __shared__ unsigned hist[kSortBins];
   for (unsigned e = threadIdx.x; e <= E; e += kSortBlock) hist[e] = 0;
-  const uint64_t first = (uint64_t)blockIdx.x * kSortTile + threadIdx.x;
-  unsigned bin[kSortItems];
+  const uint64_t first = (uint64_t)blockIdx.x * (kSortBlock * ITEMS) + threadIdx.x;
+  unsigned bin[ITEMS];
 #pragma unroll
-  for (unsigned s = 0; s < kSortItems; ++s)
+  for (unsigned s = 0; s < ITEMS; ++s)
     bin[s] = first + s * kSortBlock < n ? bin_of(experts, first + s * kSortBlock, E) : kSortBins;
   __syncthreads();
 #pragma unroll
-  for (unsigned s = 0; s < kSortItems; ++s)
+  for (unsigned s = 0; s < ITEMS; ++s)
     if (bin[s] < kSortBins) atomicAdd(&hist[bin[s]], 1u);
   __syncthreads();
   for (unsigned e = threadIdx.x; e <= E; e += kSortBlock) counts[(uint64_t)blockIdx.x * (E + 1) + e] = hist[e];
@@ -87,10 +85,10 @@ __global__ __launch_bounds__(kSortBlock) void k_route_scan(unsigned* __restrict_
 
 // Places of a tile's choices. A wavefront owns neighbouring ones and takes them 64 at a time: lanes of the same bin find each
 // other by comparing the bits of their bins, so a choice's rank among its wavefront's is known without atomics; ranks begin
-// where the earlier wavefronts', tiles' and bins' choices end. 16 choices take 2.8 us, 15,009 of 61 experts 3.1 + 6.5 (counts and
-// places), 262,144 of 256 4.8 + 10.5: a chain of steps that each wait for the one before, on as many compute units as there are tiles
-// (every workgroup counting all choices itself instead of a launch for the counts: 12,000 of few experts a microsecond less, half
-// of them of one expert twice the time, for the atomics on one counter).
+// where the earlier wavefronts', tiles' and bins' choices end. 16 choices take 2.8 us, 15,009 of 64 experts 6.8 with their counts,
+// 262,144 of 256 13.3: a chain of steps that each wait for the one before, on as many compute units as there are tiles (every workgroup
+// counting all choices itself instead of a launch for the counts: twice the time where half of them are of one expert, for the atomics
+// on one counter).
 template <typename I, unsigned ITEMS>
 __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict__ experts, uint64_t n, unsigned E,
                                                              const unsigned* __restrict__ counts, unsigned tiles,
@@ -433,6 +431,19 @@ unsigned row_grid(uint64_t tokens, unsigned lanes_log2) {
   return grid_for(tokens, kRowBlock >> lanes_log2, 1u << 22);
 }
 
+// How a sort is cut into tiles: 1, 2 or 4 choices to each of a workgroup's 1,024 lanes. One tile, and one launch, up to 4,096. From
+// there on as small tiles as there may be, for a tile's steps are what takes the time (15,009 choices of 64 experts: 6.8 us
+// with one choice to a lane, 7.5 with two, 9.5 with four; 262,144 of 256: 13.3 with two, 13.7 with four), until adding up the tiles' counts
+// takes longer (524,288 of 256: 21.2, 15.4, 16.9; 1,048,576 of 64: two 22.9, four 16.3).
+struct SortCut {
+  unsigned items;
+  uint64_t tiles;
+  explicit SortCut(uint64_t n) {
+    items = n <= 4096 ? (n <= 1024 ? 1 : n <= 2048 ? 2 : 4) : n <= 131072 ? 1 : n <= 524288 ? 2 : 4;
+    tiles = n ? (n + kSortBlock * items - 1) / (kSortBlock * items) : 1;
+  }
+};
+
 // Most lanes of a token whose row is copied or summed: a workgroup's where there are few tokens (512 x 4 rows of 4,096 bf16: 5.9 us,
 // with two wavefronts 6.7), two wavefronts otherwise (32,768 x 8 of 2,048: 236 and 227).
 unsigned lanes_of(uint64_t tokens) { return tokens < 2048 ? kRowBlock : 128; }
@@ -456,8 +467,9 @@ using namespace pskv;
   } while (0)
 
 extern "C" size_t pskv_route_room(size_t n, size_t E) {
-  if (n <= kSortTile || n > 0x7fffffffull || E > PSKV_ROUTE_MAX_EXPERTS) return 0;
-  return ((n + kSortTile - 1) / kSortTile + 1) * (E + 1) * sizeof(unsigned);
+  if (n > 0x7fffffffull || E > PSKV_ROUTE_MAX_EXPERTS) return 0;
+  const SortCut cut(n);
+  return cut.tiles == 1 ? 0 : (cut.tiles + 1) * (E + 1) * sizeof(unsigned);
 }
 
 extern "C" int pskv_route_sort(int device, void* stream, const void* experts, int index_bits, size_t n, size_t E,
@@ -483,20 +495,32 @@ extern "C" int pskv_route_sort(int device, void* stream, const void* experts, in
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const unsigned tiles = n <= kSortTile ? 1u : (unsigned)((n + kSortTile - 1) / kSortTile);
+  const SortCut cut(n);
+  const unsigned tiles = (unsigned)cut.tiles;
   const bool scanned = tiles * (E + 1) > kSortFew;
   unsigned* counts = static_cast<unsigned*>(work);
-  auto go = [&](auto* e) {
+  auto go = [&](auto* e, auto items) {
     using I = std::remove_const_t<std::remove_pointer_t<decltype(e)>>;
-    if (tiles > 1) hipLaunchKernelGGL(k_route_count<I>, dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts);
-    if (tiles > 1 && scanned) hipLaunchKernelGGL(k_route_scan, dim3((unsigned)E / 64 + 1), dim3(kSortBlock), 0, st, counts, tiles, (unsigned)E + 1);
-    hipLaunchKernelGGL((n <= kSortBlock ? k_route_place<I, 1> : k_route_place<I, kSortItems>), dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts, tiles, scanned,
-                       order, place, offsets);
+    constexpr unsigned ITEMS = decltype(items)::value;
+    if (tiles > 1) {
+      hipLaunchKernelGGL((k_route_count<I, ITEMS>), dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts);
+      if (scanned) hipLaunchKernelGGL(k_route_scan, dim3((unsigned)E / 64 + 1), dim3(kSortBlock), 0, st, counts, tiles, (unsigned)E + 1);
+    }
+    hipLaunchKernelGGL((k_route_place<I, ITEMS>), dim3(tiles), dim3(kSortBlock), 0, st, e, (uint64_t)n, (unsigned)E, counts, tiles,
+                       scanned, order, place, offsets);
+  };
+  auto with_items = [&](auto* e) {
+    if (cut.items == 1)
+      go(e, std::integral_constant<unsigned, 1>());
+    else if (cut.items == 2)
+      go(e, std::integral_constant<unsigned, 2>());
+    else
+      go(e, std::integral_constant<unsigned, 4>());
   };
   if (index_bits == 64)
-    go(static_cast<const int64_t*>(experts));
+    with_items(static_cast<const int64_t*>(experts));
   else
-    go(static_cast<const int32_t*>(experts));
+    with_items(static_cast<const int32_t*>(experts));
   PSKV_HIP(hipGetLastError());
   return PSKV_OK;
 }

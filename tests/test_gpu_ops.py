@@ -81,7 +81,7 @@ def sort(ops, experts, E, **more):
 @pytest.mark.parametrize("bits", [32, 64])
 @pytest.mark.parametrize("T,K,E", [(0, 2, 5), (1, 1, 1), (1, 2, 2048), (7, 3, 2), (64, 1, 7), (65, 8, 63), (1000, 3, 64), (513, 5, 65),
                                    (1024, 8, 256), (8193, 1, 8), (1025, 1, 8), (4096, 1, 9), (4097, 1, 300), (4099, 6, 1000), (2731, 3, 2048), (100003, 3, 60),
-                                   (262145, 1, 1), (600007, 1, 2047)])
+                                   (2048, 1, 20), (131072, 1, 33), (131073, 1, 70), (524289, 1, 3), (262145, 1, 1), (600007, 1, 2047)])
 @pytest.mark.parametrize("lost", [0.0, 0.3, 1.0])
 def test_sort(ops, dev, bits, T, K, E, lost):
     import torch
