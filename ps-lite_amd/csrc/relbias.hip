@@ -272,12 +272,12 @@ constexpr unsigned kCols = 64 * kWide;  // of a wavefront
 
 // The same the other way round: rows are summed over the batch, then along the diagonals, which move up one lane every
 // eight rows; those that leave lane 63 and those that are there in the end are summed by bucket, 64 neighbouring diagonals
-// at a time. Every sum has one order. partial[head][bucket][workgroup of the head], or the gradient itself where a head has one
+// at a time. Every sum has one order. `to`: [head][bucket][workgroup of the head], or the gradient itself where a head has one
 // workgroup. 8 x 16 x 1024 x 1024 bf16: 45 us, 6.0 TB/s, and 5 for
 // k_relbias_join (a lane to a diagonal, element by element: 460).
 template <typename T, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ grad, const int64_t* __restrict__ q_at,
-                                                          float* __restrict__ partial, float* __restrict__ grad_table,
+                                                          float* __restrict__ to, uint64_t by_head, uint64_t by_bucket,
                                                           unsigned buckets, unsigned tiles, Cut cut, Shape s, Buckets b) {
   __shared__ uint32_t border[kMostBuckets / 2 + 1];
   __shared__ float diagonal[kWaves][kMostRows + kCols];
@@ -346,13 +346,15 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
       run = 0.0f;
       now = kMostBuckets;
     };
-    auto sum_up = [&](unsigned u, float sum) {
-      const unsigned first = __builtin_amdgcn_readfirstlane(u);
+    for (unsigned x0 = 0; x0 < reached; x0 += 64) {
+      const unsigned x = x0 + lane;
+      float sum = x < reached ? diagonal[wave][x] : 0.0f;
+      const unsigned u = bucket_of(b, border, rel + (int)x), first = __builtin_amdgcn_readfirstlane(u);
       if (__all(u == first)) {
         if (first != now) finish();
         now = first;
         run += sum;
-        return;
+        continue;
       }
       finish();
       // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
@@ -360,22 +362,6 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
       sum = sum_along(sum, lane == 0 || below != u ? 1 : 0);
       if (lane == 63 || above != u) sums[wave][u] += sum;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    };
-    const unsigned first = bucket_of(b, border, rel), last = bucket_of(b, border, rel + (int)reached - 1);
-    if (first == last) {  // a tile far from the main diagonal: so have all between
-      now = first;
-      for (unsigned x = lane; x < reached; x += 64) run += diagonal[wave][x];
-    } else {
-      unsigned next_u = bucket_of(b, border, rel + (int)lane);
-      float next = lane < reached ? diagonal[wave][lane] : 0.0f;
-      for (unsigned x = lane; x - lane < reached;) {
-        const unsigned u = next_u;
-        const float part = next;
-        x += 64;  // (looked up while the ones before are summed)
-        next = x < reached ? diagonal[wave][x] : 0.0f;
-        next_u = bucket_of(b, border, rel + (int)x);
-        sum_up(u, part);
-      }
     }
     finish();
   }
@@ -384,10 +370,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     float sum = sums[0][u];
 #pragma unroll
     for (unsigned w = 1; w < kWaves; ++w) sum += sums[w][u];
-    if (gridDim.x == 1)
-      grad_table[u * s.H + head] = sum;
-    else
-      partial[(head * buckets + u) * gridDim.x + blockIdx.x] = sum;
+    to[head * by_head + u * by_bucket + blockIdx.x] = sum;
   }
 }
 
@@ -615,7 +598,8 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
       // (of several gradients of 83 MB in turn, 31 us each, some is still in the memory-side cache, 34 past it; of 134 MB 32 and 29)
       auto kernel = B * H * Q * K * sizeof(T) > kPastBytes / 2 ? k_relbias_sums<T, true> : k_relbias_sums<T, false>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad),
-                         q_at, partial, grad_table, (unsigned)buckets, (unsigned)cut.tiles(), cut, s, b);
+                         q_at, groups == 1 ? grad_table : partial, groups == 1 ? (uint64_t)1 : buckets * groups,
+                         groups == 1 ? (uint64_t)H : groups, (unsigned)buckets, (unsigned)cut.tiles(), cut, s, b);
     });
   if (groups != 1)
     hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(64), 0, st, partial, (unsigned)buckets,
