@@ -212,10 +212,12 @@ __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict_
 // next call wants (36 MB past it: 8.4 -> 10.8 us out, 8.9 -> 9.7 back).
 constexpr unsigned kRowBlock = 256;
 
+// (Kernels with up to 104 bytes of arguments that do not ask for the size of their grid take the calling thread 2.7 us to launch, others 3.3.)
 struct RowArgs {
-  uint64_t tokens, k, rows;      // rows: of the sorted side
   uint64_t token_stride, row_stride;  // elements
-  unsigned choices, lanes_log2;
+  uint32_t tokens, k, rows;           // rows: of the sorted side
+  uint32_t choices, lanes_log2;
+  uint32_t groups;  // workgroups of the launch
 };
 
 // The token of a lane; where a wavefront or more serves one, the compiler is told that all lanes have the same, so that places and
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_rows(const T* __restrict__ 
   using Vec = typename Row<T>::Vec;
   constexpr unsigned W = Row<T>::kWide;
   const unsigned lanes = 1u << a.lanes_log2;
-  const uint64_t per = (uint64_t)gridDim.x * (kRowBlock >> a.lanes_log2);
+  const uint64_t per = (uint64_t)a.groups * (kRowBlock >> a.lanes_log2);
   for (uint64_t t = token_of<ONE>(((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2); t < a.tokens; t += per) {
     const T* from = x + t * a.token_stride;
     const int* at = place + t * a.choices;
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ r
   using Vec = typename Row<T>::Vec;
   constexpr unsigned W = Row<T>::kWide, kAhead = 8;
   const unsigned lanes = 1u << a.lanes_log2;
-  const uint64_t per = (uint64_t)gridDim.x * (kRowBlock >> a.lanes_log2);
+  const uint64_t per = (uint64_t)a.groups * (kRowBlock >> a.lanes_log2);
   for (uint64_t t = token_of<ONE>(((uint64_t)blockIdx.x * kRowBlock + threadIdx.x) >> a.lanes_log2); t < a.tokens; t += per) {
     const int* at = place + t * a.choices;
     const float* w = weights ? weights + t * a.choices : nullptr;
@@ -328,11 +330,11 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum_grad(const T* __restric
   constexpr unsigned W = Row<T>::kWide, C = kKept / NV;
   const unsigned lanes = 1u << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const uint64_t per = kRowBlock >> a.lanes_log2;
-  const uint64_t wide = (uint64_t)lanes * W, whole = a.k / W * W;  // elements of a vector for all lanes; of whole vectors
+  const uint64_t wide = (uint64_t)lanes * W, whole = (uint64_t)a.k / W * W;  // elements of a vector for all lanes; of whole vectors
   const unsigned parts = (a.choices + share - 1) / share;
-  const uint64_t units = a.tokens * parts;
+  const uint64_t units = (uint64_t)a.tokens * parts;
   // (lanes of one unit add up together, and leave together)
-  for (uint64_t u = token_of<ONE>(blockIdx.x * per + (threadIdx.x >> a.lanes_log2)); u < units; u += gridDim.x * per) {
+  for (uint64_t u = token_of<ONE>(blockIdx.x * per + (threadIdx.x >> a.lanes_log2)); u < units; u += a.groups * per) {
     const unsigned t = (unsigned)u / parts, j0 = ((unsigned)u - t * parts) * share;
     const unsigned end = a.choices - j0 < share ? a.choices : j0 + share;
     const T* g = grad + t * a.token_stride;
@@ -427,10 +429,6 @@ int check_stride(const char* what, uint64_t n, uint64_t k, uint64_t stride, bool
   return PSKV_OK;
 }
 
-unsigned row_grid(uint64_t tokens, unsigned lanes_log2) {
-  return grid_for(tokens, kRowBlock >> lanes_log2, 1u << 22);
-}
-
 // How a sort is cut into tiles: 1, 2 or 4 choices to each of a workgroup's 1,024 lanes. One tile, and one launch, up to 4,096. From
 // there on as small tiles as there may be, for a tile's steps are what takes the time (15,009 choices of 64 experts: 6.8 us
 // with one choice to a lane, 7.5 with two, 9.5 with four; 262,144 of 256: 13.3 with two, 13.7 with four), until adding up the tiles' counts
@@ -452,7 +450,9 @@ RowArgs row_args(uint64_t tokens, uint64_t choices, uint64_t rows, uint64_t k, u
                  int type, unsigned most_lanes) {
   const uint64_t wide = 16 / type_bytes(type);
   const unsigned lanes = lanes_for((k + wide - 1) / wide, most_lanes);
-  return RowArgs{tokens, k, rows, token_stride, row_stride, (unsigned)choices, (unsigned)__builtin_ctz(lanes)};
+  const unsigned lanes_log2 = (unsigned)__builtin_ctz(lanes);
+  return RowArgs{token_stride, row_stride, (uint32_t)tokens, (uint32_t)k, (uint32_t)rows, (uint32_t)choices, lanes_log2,
+                 grid_for(tokens, kRowBlock >> lanes_log2, 1u << 22)};
 }
 
 }  // namespace
@@ -544,7 +544,7 @@ extern "C" int pskv_route_rows(int device, void* stream, int type, const void* x
     with_flag((1 + choices) * tokens * k * size > kPastBytes, [&](auto far) {
       constexpr bool PAST = decltype(far)::value;
       auto kernel = a.lanes_log2 >= 6 ? k_route_rows<T, true, PAST> : k_route_rows<T, false, PAST>;
-      hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+      hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(kRowBlock), 0,
                          static_cast<hipStream_t>(stream), static_cast<const T*>(x), place, static_cast<T*>(rows), a);
     });
   });
@@ -573,7 +573,7 @@ extern "C" int pskv_route_sum(int device, void* stream, int type, const void* ro
     with_flag((1 + choices) * tokens * k * size > kPastBytes, [&](auto far) {
       constexpr bool PAST = decltype(far)::value;
       auto kernel = a.lanes_log2 >= 6 ? k_route_sum<T, true, PAST> : k_route_sum<T, false, PAST>;
-      hipLaunchKernelGGL(kernel, dim3(row_grid(tokens, a.lanes_log2)), dim3(kRowBlock), 0,
+      hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(kRowBlock), 0,
                          static_cast<hipStream_t>(stream), static_cast<const T*>(rows), place, weights, static_cast<T*>(out), a);
     });
   });
@@ -601,11 +601,11 @@ extern "C" int pskv_route_sum_grad(int device, void* stream, int type, const voi
     return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
-  const RowArgs a = row_args(tokens, choices, n_rows, k, grad_stride, rows_stride, type, 64);
+  RowArgs a = row_args(tokens, choices, n_rows, k, grad_stride, rows_stride, type, 64);
   // (300 tokens x 8 choices of 1,024 bf16: all of a token in one wavefront 14.2 us, in eight 5.6)
   unsigned share = (unsigned)choices;
   while (share > 1 && ((tokens * ((choices + share - 1) / share)) << a.lanes_log2) < 64 * 4096) share = (share + 1) / 2;
-  const uint64_t units = tokens * ((choices + share - 1) / share);
+  a.groups = grid_for(tokens * ((choices + share - 1) / share), kRowBlock >> a.lanes_log2, 1u << 22);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     with_flag((1 + 2 * choices) * tokens * k * size > kPastBytes, [&](auto far) {
@@ -616,7 +616,7 @@ extern "C" int pskv_route_sum_grad(int device, void* stream, int type, const voi
                     : vectors <= 128     ? k_route_sum_grad<T, true, PAST, 2, false>
                     : vectors <= 4 * 64 ? k_route_sum_grad<T, true, PAST, 4, false>
                                          : k_route_sum_grad<T, true, PAST, 4, true>;
-      hipLaunchKernelGGL(kernel, dim3(row_grid(units, a.lanes_log2)), dim3(kRowBlock), 0,
+      hipLaunchKernelGGL(kernel, dim3(a.groups), dim3(kRowBlock), 0,
                          static_cast<hipStream_t>(stream), static_cast<const T*>(grad), static_cast<const T*>(rows), place, weights,
                          static_cast<T*>(grad_rows), (uint64_t)grad_rows_stride, grad_weights, share, a);
     });
