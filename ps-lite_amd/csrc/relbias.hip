@@ -265,7 +265,125 @@ __global__ __launch_bounds__(kBlock) void k_relbias_step(const float* __restrict
   }
 }
 
+// --- narrow matrices ---------------------------------------------------------------------------------------------
+
+// A wavefront whose lanes are one row's columns has little to do where there are few of them. There a workgroup takes a plane: as
+// many whole rows as kPlane elements hold, its lanes going through them cell by cell, 2 or 4 bytes at a time. That costs by the
+// cell: 16.8 M of them in 1,024 matrices take the bias of scores 27 to 30 us, alone 24, the gradient in bf16 28 to 30 and in
+// float32 17, and 45 and 36 where each sequence has its own position. By columns they take (bf16; 1, 16, 49 of them)
+//     scores 2306, 160, 66   alone 1363, 90, 36   gradient 1170, 64, 49   own positions 1927, 113, 58
+// and less than by planes from where these rules end (bf16, float32; planes behind the arrow):
+//     scores in bf16, 112 columns: 29.6 -> 26.2; 120: 27.1 -> 28.5   in float32, 80: 29.4 -> 28.8; 96: 27.4 -> 28.5
+//     alone, 63: 34 -> 24, 29 -> 24; 64, whose rows begin at whole lines: 27.8 -> 24.9, 22.1 -> 24.5; 80: 23.5 -> 24.8, 19.0 -> 23.9
+//     gradient, 120: 30.8 -> 28.2, 35 -> 17 (80, whose rows do so in bf16: 26.3 -> 28.7, 31.7 -> 16.8); 128: 19.6 -> 28.3, 22.5 -> 16.7
+//     own positions, 63: 56 -> 46, 58 -> 36; 64: 31 -> 47, 35 -> 36
+constexpr unsigned kPlane = 2048;
+constexpr unsigned kEach = kPlane / kBlock;  // cells of a lane
+bool by_planes(size_t Q, size_t K, size_t size, bool scores) { return Q > 1 && K <= (!scores ? 63 : size == 2 ? 112 : 80); }
+bool sums_by_planes(size_t K, bool own_positions) { return K <= (own_positions ? 63 : 127); }
+
+struct Plane {
+  unsigned row[kEach], col[kEach];  // (of cells that are not there: the first)
+  unsigned passes, cells;           // the same for the workgroup
+  __device__ __forceinline__ Plane(unsigned rows, unsigned K) {
+    cells = rows * K;
+    passes = (cells + kBlock - 1) / kBlock;
+    const unsigned down = kBlock / K, along = kBlock - down * K;
+    unsigned r = threadIdx.x / K, k = threadIdx.x - r * K;
+#pragma unroll
+    for (unsigned i = 0; i < kEach; ++i) {
+      row[i] = has(i) ? r : 0;
+      col[i] = has(i) ? k : 0;
+      r += down, k += along;
+      if (k >= K) k -= K, ++r;
+    }
+  }
+  __device__ __forceinline__ bool has(unsigned i) const { return threadIdx.x + i * kBlock < cells; }
+};
+
+// The bias of a plane's diagonals, looked up once for all its batches.
+template <typename T, bool SCORES>
+__global__ __launch_bounds__(kBlock) void k_relbias_narrow(const float* __restrict__ table, const int64_t* __restrict__ q_at,
+                                                            const T* scores, T* out, unsigned tiles, Cut cut, Shape s, Buckets b) {
+  __shared__ uint32_t border[kMostBuckets / 2 + 1];
+  __shared__ float bias[kPlane];  // (rows + K - 1 <= rows K)
+  fetch_borders(border, b);
+  const unsigned K = (unsigned)s.K;
+  for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const Tile t(tile, cut, s);
+    const Plane c(t.rows, K);
+    const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) - t.r0 - (t.rows - 1)));
+    __syncthreads();
+    for (unsigned x = threadIdx.x; x < t.rows + K - 1; x += kBlock)
+      bias[x] = table[bucket_of(b, border, rel + (int)x) * (unsigned)s.H + t.head0];
+    __syncthreads();
+    const T* from = SCORES ? scores + t.batch0 * s.in[0] + t.head0 * s.in[1] + t.r0 * s.in[2] : nullptr;
+    T* to = out + t.batch0 * s.out[0] + t.head0 * s.out[1] + t.r0 * s.out[2];
+    float v[kEach];
+#pragma unroll
+    for (unsigned i = 0; i < kEach; ++i) v[i] = c.has(i) ? bias[t.rows - 1 + c.col[i] - c.row[i]] : 0.0f;
+    for (unsigned n = 0; n < t.batches; ++n) {
+      T x[kEach];
+      if (SCORES) {
+#pragma unroll
+        for (unsigned i = 0; i < kEach; ++i)
+          if (i < c.passes) x[i] = from[n * s.in[0] + c.row[i] * s.in[2] + c.col[i]];
+      }
+#pragma unroll
+      for (unsigned i = 0; i < kEach; ++i)
+        if (c.has(i)) to[n * s.out[0] + c.row[i] * s.out[2] + c.col[i]] = (T)(SCORES ? (float)x[i] + v[i] : v[i]);
+    }
+  }
+}
+
 // --- the gradient ------------------------------------------------------------------------------------------------
+
+// Adds diagonals x of `from`, `from` + `step`, ... below `count`, 64 neighbours at a time, to a wavefront's sums of their buckets;
+// `rel` is diagonal 0's relative position. Far from the main diagonal 64 of them have one bucket: those are added up lane by lane
+// until another one comes.
+template <typename F>
+__device__ __forceinline__ void add_buckets(float* sums, const Buckets& b, const uint32_t* border, int32_t rel, unsigned from,
+                                            unsigned step, unsigned count, F value) {
+  const unsigned lane = threadIdx.x & 63;
+  float run = 0.0f;
+  unsigned now = kMostBuckets;
+  auto finish = [&] {
+    if (now == kMostBuckets) return;
+    run = sum_along(run, 0);
+    if (lane == 63) sums[now] += run;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    run = 0.0f;
+    now = kMostBuckets;
+  };
+  for (unsigned x0 = from; x0 < count; x0 += step) {
+    const unsigned x = x0 + lane;
+    float sum = x < count ? value(x) : 0.0f;
+    const unsigned u = bucket_of(b, border, rel + (int)x), first = __builtin_amdgcn_readfirstlane(u);
+    if (__all(u == first)) {
+      if (first != now) finish();
+      now = first;
+      run += sum;
+      continue;
+    }
+    finish();
+    // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
+    const unsigned below = dpp<0x138 /* wave_shr:1 */, 0xf>(u), above = dpp<0x130 /* wave_shl:1 */, 0xf>(u);
+    sum = sum_along(sum, lane == 0 || below != u ? 1 : 0);
+    if (lane == 63 || above != u) sums[u] += sum;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  finish();
+}
+
+// The wavefronts' sums of a workgroup. (Behind a barrier.)
+__device__ __forceinline__ void put_sums(const float (&sums)[kWaves][kMostBuckets], float* to, uint64_t by_bucket, unsigned buckets) {
+  for (unsigned u = threadIdx.x; u < buckets; u += kBlock) {
+    float sum = sums[0][u];
+#pragma unroll
+    for (unsigned w = 1; w < kWaves; ++w) sum += sums[w][u];
+    to[u * by_bucket] = sum;
+  }
+}
 
 constexpr unsigned kWide = 8;           // neighbouring columns of a lane
 constexpr unsigned kCols = 64 * kWide;  // of a wavefront
@@ -335,43 +453,65 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0 - reach));
     // (those that no element of the tile is on are left out)
     const unsigned reached = reach + (s.K - t.c0 < kCols ? (unsigned)(s.K - t.c0) : kCols);
-    // Far from the main diagonal 64 of them have one bucket: those are added up lane by lane until another one comes.
-    float run = 0.0f;
-    unsigned now = kMostBuckets;
-    auto finish = [&] {
-      if (now == kMostBuckets) return;
-      run = sum_along(run, 0);
-      if (lane == 63) sums[wave][now] += run;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      run = 0.0f;
-      now = kMostBuckets;
-    };
-    for (unsigned x0 = 0; x0 < reached; x0 += 64) {
-      const unsigned x = x0 + lane;
-      float sum = x < reached ? diagonal[wave][x] : 0.0f;
-      const unsigned u = bucket_of(b, border, rel + (int)x), first = __builtin_amdgcn_readfirstlane(u);
-      if (__all(u == first)) {
-        if (first != now) finish();
-        now = first;
-        run += sum;
-        continue;
-      }
-      finish();
-      // lanes of one bucket are neighbours: a sum over each stretch of them, left at its last lane
-      const unsigned below = dpp<0x138 /* wave_shr:1 */, 0xf>(u), above = dpp<0x130 /* wave_shl:1 */, 0xf>(u);
-      sum = sum_along(sum, lane == 0 || below != u ? 1 : 0);
-      if (lane == 63 || above != u) sums[wave][u] += sum;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    finish();
+    add_buckets(sums[wave], b, border, rel, 0, 64, reached, [&](unsigned x) { return diagonal[wave][x]; });
   }
   __syncthreads();
-  for (unsigned u = threadIdx.x; u < buckets; u += kBlock) {
-    float sum = sums[0][u];
+  put_sums(sums, to + head * by_head + blockIdx.x, by_bucket, buckets);
+}
+
+// Of narrow matrices: a workgroup sums a plane over its batches, and a lane each diagonal of the sums. An odd number of
+// columns apart, the rows' elements that neighbouring diagonals begin with are in banks of their own.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_relbias_narrow_sums(const T* __restrict__ grad, const int64_t* __restrict__ q_at,
+                                                                 float* __restrict__ to, uint64_t by_head, uint64_t by_bucket,
+                                                                 unsigned buckets, Cut cut, Shape s, Buckets b) {
+  constexpr unsigned kAhead = 4;  // batches asked for at a time
+  __shared__ uint32_t border[kMostBuckets / 2 + 1];
+  __shared__ float plane[kPlane];
+  __shared__ float sums[kWaves][kMostBuckets];
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint64_t head = blockIdx.y;
+  fetch_borders(border, b);
+  for (unsigned u = lane; u < buckets; u += 64) sums[wave][u] = 0.0f;
+  const Tile t(blockIdx.x, cut, s);  // (of any head: cut.parts is 1)
+  const Plane c(t.rows, (unsigned)s.K);
+  const T* from = grad + t.batch0 * s.in[0] + head * s.in[1] + t.r0 * s.in[2];
+  float sum[kEach] = {};
+  auto some = [&](unsigned n0, auto count) {
+    constexpr unsigned N = decltype(count)::value;
+    T x[N][kEach];
 #pragma unroll
-    for (unsigned w = 1; w < kWaves; ++w) sum += sums[w][u];
-    to[head * by_head + u * by_bucket + blockIdx.x] = sum;
-  }
+    for (unsigned n = 0; n < N; ++n)
+#pragma unroll
+      for (unsigned i = 0; i < kEach; ++i)
+        if (i < c.passes) x[n][i] = from[(n0 + n) * s.in[0] + c.row[i] * s.in[2] + c.col[i]];
+#pragma unroll
+    for (unsigned n = 0; n < N; ++n)
+#pragma unroll
+      for (unsigned i = 0; i < kEach; ++i)
+        if (i < c.passes) sum[i] += (float)x[n][i];
+  };
+  unsigned n = 0;
+  for (; n + kAhead <= t.batches; n += kAhead) some(n, std::integral_constant<unsigned, kAhead>());
+  for (; n < t.batches; ++n) some(n, std::integral_constant<unsigned, 1>());
+  const unsigned K = (unsigned)s.K, pitch = K | 1;
+#pragma unroll
+  for (unsigned i = 0; i < kEach; ++i)
+    if (c.has(i)) plane[c.row[i] * pitch + c.col[i]] = sum[i];
+  __syncthreads();
+  // diagonal x begins at column x - (rows - 1) of row 0, or at column 0 of row rows - 1 - x
+  const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) - t.r0 - (t.rows - 1)));
+  add_buckets(sums[wave], b, border, rel, wave * 64, kBlock, t.rows + K - 1, [&](unsigned x) {
+    const unsigned r = x < t.rows ? t.rows - 1 - x : 0, k = x < t.rows ? 0 : x - (t.rows - 1);
+    const unsigned cells = t.rows - r < K - k ? t.rows - r : K - k;
+    const float* at = plane + r * pitch + k;
+    float along = 0.0f;
+#pragma unroll 8
+    for (unsigned i = 0; i < cells; ++i) along += at[i * (pitch + 1)];
+    return along;
+  });
+  __syncthreads();
+  put_sums(sums, to + head * by_head + blockIdx.x, by_bucket, buckets);
 }
 
 // The workgroups' sums of a bucket and head: a wavefront to each.
@@ -459,6 +599,22 @@ Cut cut_for_bias(size_t B, size_t H, size_t Q, size_t K, size_t size) {
   return c;
 }
 
+// Of either: the planes of narrow matrices, for as many batches as there are workgroups without to fill the GPU.
+Cut cut_for_planes(size_t B, size_t heads, size_t Q, size_t K, bool own_positions) {
+  Cut c{};
+  c.cols = (unsigned)K;
+  c.rows = kPlane / ((unsigned)K | 1);
+  if (c.rows > Q) c.rows = (unsigned)Q;
+  c.across = c.heads = c.parts = 1;
+  c.strips = (unsigned)((Q + c.rows - 1) / c.rows);
+  c.batches = own_positions ? 1 : (unsigned)B;
+  for (;;) {
+    c.chunks = (unsigned)((B + c.batches - 1) / c.batches);
+    if (c.batches == 1 || c.tiles() * heads >= kFilled) return c;
+    c.batches = (c.batches + 1) / 2;
+  }
+}
+
 // Of the gradient: the tiles of a head. Enough wavefronts to fill the GPU, if that can be had: fewer rows for each first, then fewer
 // batches, then fewer rows again (64 rows as long as there are batches to share out: 16 x 2048 x 2048 bf16 28 us, from 32 rows on 32).
 Cut cut_for_sums(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
@@ -485,8 +641,23 @@ Cut cut_for_sums(size_t B, size_t H, size_t Q, size_t K, bool own_positions) {
   return c;
 }
 
-// The workgroups of a head.
-uint64_t groups_of(const Cut& c) { return (c.tiles() + kWaves - 1) / kWaves; }
+// How the gradient is cut up, and the workgroups of a head.
+struct SumsCut {
+  bool narrow;
+  Cut cut;
+  uint64_t groups;
+  SumsCut(size_t B, size_t H, size_t Q, size_t K, bool own_positions) : narrow(sums_by_planes(K, own_positions)) {
+    if (narrow) {
+      cut = cut_for_planes(B, H, Q, K, own_positions);
+      groups = cut.tiles();
+      narrow = groups <= 1u << 20;  // (beyond, smaller working memory counts)
+    }
+    if (!narrow) {
+      cut = cut_for_sums(B, H, Q, K, own_positions);
+      groups = (cut.tiles() + kWaves - 1) / kWaves;
+    }
+  }
+};
 
 }  // namespace
 }  // namespace pskv
@@ -531,17 +702,21 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
     if (!same && a < o + out_bytes && o < a + extent(scores_stride, s, size))
       return set_error(PSKV_EINVAL, "out lies in the scores and is not the same tensor");
   }
-  const Cut cut = cut_for_bias(B, H, Q, K, type_bytes(type));
+  const bool narrow = by_planes(Q, K, type_bytes(type), scores != nullptr);
+  Cut cut = narrow ? cut_for_planes(B, H, Q, K, q_at != nullptr) : cut_for_bias(B, H, Q, K, type_bytes(type));
+  if (narrow) cut.heads = 1, cut.parts = (unsigned)H;
   if (cut.tiles() > kMostTiles) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   with_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles(), kWaves, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream),
+      hipLaunchKernelGGL(kernel, dim3(grid_for(cut.tiles(), narrow ? 1 : kWaves, 1u << 22)), dim3(kBlock), 0, static_cast<hipStream_t>(stream),
                          table, q_at, static_cast<const T*>(scores), static_cast<T*>(out), (unsigned)cut.tiles(), cut, s, b);
     };
-    if (Q == 1)
+    if (narrow)
+      launch(scores ? k_relbias_narrow<T, true> : k_relbias_narrow<T, false>);
+    else if (Q == 1)
       launch(scores ? k_relbias_step<T, true> : k_relbias_step<T, false>);
     else if (B * H * Q * K * sizeof(T) * (scores ? 2 : 1) > kPastBytes)
       launch(scores ? k_relbias<T, true, true> : k_relbias<T, false, true>);
@@ -554,7 +729,7 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
 
 extern "C" size_t pskv_relbias_grad_room(size_t buckets, size_t H, size_t B, size_t Q, size_t K, int own_positions) {
   if (B == 0 || Q == 0 || K == 0 || B > (1u << 20) || Q > (1u << 20) || K > (1u << 30)) return 0;
-  const uint64_t groups = groups_of(cut_for_sums(B, H, Q, K, own_positions != 0));
+  const uint64_t groups = SumsCut(B, H, Q, K, own_positions != 0).groups;
   return groups == 1 ? 0 : groups * buckets * H * sizeof(float);
 }
 
@@ -570,14 +745,17 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
   if (!grad_table) return set_error(PSKV_EINVAL, "null buffer");
   Shape s{B, H, Q, K, k_first - q_first, {0, 0, 0}, {0, 0, 0}};
   const bool any = B && Q && K;
+  bool narrow = false;
   Cut cut{};
   uint64_t groups = 0;
   if (any) {
     if (!grad) return set_error(PSKV_EINVAL, "null buffer");
     if ((rc = check_strides("grad", grad_stride, s, false))) return rc;
     for (int i = 0; i < 3; ++i) s.in[i] = (uint64_t)grad_stride[i];
-    cut = cut_for_sums(B, H, Q, K, q_at != nullptr);
-    groups = groups_of(cut);
+    const SumsCut sums(B, H, Q, K, q_at != nullptr);
+    narrow = sums.narrow;
+    cut = sums.cut;
+    groups = sums.groups;
     if (groups > kMostTiles / kBlock) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");
     const size_t room = groups == 1 ? 0 : groups * buckets * H * sizeof(float);
     if (room == 0)
@@ -595,11 +773,18 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
   if (any)
     with_type(type, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
+      auto launch = [&](auto kernel, auto... tiles) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad), q_at,
+                           groups == 1 ? grad_table : partial, groups == 1 ? (uint64_t)1 : buckets * groups,
+                           groups == 1 ? (uint64_t)H : groups, (unsigned)buckets, tiles..., cut, s, b);
+      };
       // (of several gradients of 83 MB in turn, 31 us each, some is still in the memory-side cache, 34 past it; of 134 MB 32 and 29)
-      auto kernel = B * H * Q * K * sizeof(T) > kPastBytes / 2 ? k_relbias_sums<T, true> : k_relbias_sums<T, false>;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)groups, (unsigned)H), dim3(kBlock), 0, st, static_cast<const T*>(grad),
-                         q_at, groups == 1 ? grad_table : partial, groups == 1 ? (uint64_t)1 : buckets * groups,
-                         groups == 1 ? (uint64_t)H : groups, (unsigned)buckets, (unsigned)cut.tiles(), cut, s, b);
+      if (narrow)
+        launch(k_relbias_narrow_sums<T>);
+      else if (B * H * Q * K * sizeof(T) > kPastBytes / 2)
+        launch(k_relbias_sums<T, true>, (unsigned)cut.tiles());
+      else
+        launch(k_relbias_sums<T, false>, (unsigned)cut.tiles());
     });
   if (groups != 1)
     hipLaunchKernelGGL(k_relbias_join, dim3((unsigned)buckets, (unsigned)H), dim3(64), 0, st, partial, (unsigned)buckets,

@@ -325,6 +325,23 @@ BIAS = [  # B, H, Q, K, buckets, far, two_sided, q_first, k_first, own positions
     (70, 1000, 1, 3, 4, 5, True, 0, 0, False),
     (64, 13, 1, 5000, 32, 128, False, 0, 0, True),
     (3, 2, 8, 513, 32, 128, True, 0, 0, True),
+    # few columns: planes of 2,048 elements, and what is behind the last of them; many batches to a workgroup; either side of 63, 80, 112 and 127
+    (9, 2, 2049, 1, 32, 128, True, 0, 0, False),
+    (6, 3, 1030, 2, 16, 300, False, 5, 0, True),
+    (1, 2, 2000, 17, 64, 1500, False, 0, 1990, False),
+    (130, 4, 49, 49, 32, 128, True, 0, 0, False),
+    (200, 70, 50, 31, 32, 40, True, 0, 0, False),
+    (2, 3, 17, 127, 256, 2000, True, 3, 1, True),
+    (3, 5, 33, 128, 32, 128, True, 0, 0, False),
+    (3, 5, 33, 129, 32, 128, True, 0, 0, False),
+    (7, 3, 1, 100, 32, 128, False, 90, 0, False),
+    (9, 2, 65, 63, 32, 128, True, 40, 0, True),
+    (3, 2, 65, 64, 32, 128, True, 40, 0, True),
+    (5, 3, 26, 80, 32, 128, True, 0, 0, False),
+    (5, 3, 26, 81, 32, 128, True, 0, 0, False),
+    (5, 3, 21, 112, 32, 128, True, 0, 0, False),
+    (5, 3, 21, 113, 32, 128, True, 0, 0, False),
+    (11, 3, 33, 127, 64, 128, False, 100, 0, False),
 ]
 
 
@@ -435,16 +452,19 @@ def test_gradient_of_many_rows(ops, dev, type, B, H, Q, K):
 
 
 @pytest.mark.parametrize("type", TYPES)
-def test_infinities_stay_in_their_bucket(ops, dev, type):
+@pytest.mark.parametrize("narrow", [False, True])
+def test_infinities_stay_in_their_bucket(ops, dev, type, narrow):
     import torch
-    announce("relbias_grad, special values", type)
-    H, Q, K = 3, 70, 613
+    announce("relbias_grad, special values", type, narrow)
+    H, Q, K = (3, 613, 70) if narrow else (3, 70, 613)
     grad = normal(seeded(4), 2, H, Q, K, type=type)
     clean = torch.empty(32, H, device=dev)
     ops.relbias_grad(grad, clean, 128)
     want = clean.clone()
     for h, i, j, value in [(0, 5, 5, float("inf")), (1, 69, 612, float("nan")), (2, 69, 0, float("-inf")), (2, 0, 3, float("inf")),
                            (0, 33, 610, float("nan"))]:
+        if narrow:
+            i, j = j, i
         grad[1, h, i, j] = value
         u = plain_bucket(j - i, 32, 128, True)
         want[u, h] = float("nan") if not np.isinf(value) or not torch.isfinite(want[u, h]) else value
@@ -674,10 +694,11 @@ def test_rows_beyond_32_bits(ops, dev):
     assert not bool(grad_rows.view(torch.int32).any())
 
 
-def test_scores_beyond_32_bits(ops, dev):
+@pytest.mark.parametrize("K", [601, 60])
+def test_scores_beyond_32_bits(ops, dev, K):
     import torch
-    announce("relbias, a batch 2^31 elements apart")
-    B, H, Q, K, apart = 3, 2, 9, 601, (1 << 31) + 24
+    announce("relbias, a batch 2^31 elements apart", K)
+    B, H, Q, apart = 3, 2, 9, (1 << 31) + 24
     whole = torch.zeros((B - 1) * apart + H * Q * K, dtype=torch.bfloat16, device=dev)
     out = whole.as_strided((B, H, Q, K), (apart, Q * K, K, 1))
     g = seeded(7)
