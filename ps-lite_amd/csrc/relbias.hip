@@ -279,8 +279,17 @@ __global__ __launch_bounds__(kBlock) void k_relbias_step(const float* __restrict
 //     own positions, 63: 56 -> 46, 58 -> 36; 64: 31 -> 47, 35 -> 36
 constexpr unsigned kPlane = 2048;
 constexpr unsigned kEach = kPlane / kBlock;  // cells of a lane
-bool by_planes(size_t Q, size_t K, size_t size, bool scores) { return Q > 1 && K <= (!scores ? 63 : size == 2 ? 112 : 80); }
-bool sums_by_planes(size_t K, bool own_positions) { return K <= (own_positions ? 63 : 127); }
+uint64_t plane_rows(size_t Q, size_t K) { return kPlane / (K | 1) < Q ? kPlane / (K | 1) : Q; }
+bool tall(size_t Q, size_t K) { return K <= kPlane / 2 && Q / ((Q + plane_rows(Q, K) - 1) / plane_rows(Q, K)) >= 28; }
+// Where each sequence has its own position, a plane is looked up or summed into buckets for one of them: what that takes, as long
+// as some 20 rows by columns, has to be worth it (8,192 or 4,096 sequences, 16 heads; scores in bf16, float32, gradient in bf16, float32):
+//     8 x 8:   159 -> 334, 112 -> 351, 239 -> 352, 266 -> 346     16 x 16: 312 -> 369, 215 -> 368, 338 -> 366, 368 -> 355
+//     30 x 30: 323 -> 209, 270 -> 250, 302 -> 222, 339 -> 191     50 x 5:  655 -> 187, 371 -> 187, 656 -> 176, 511 -> 174
+// (49 x 49, two planes of 24 rows, 2,048 sequences: 314 -> 283, 239 -> 309, 246 -> 297, 257 -> 244).
+bool by_planes(size_t Q, size_t K, size_t size, bool scores, bool own_positions) {
+  return Q > 1 && K <= (!scores ? 63 : size == 2 ? 112 : 80) && (!own_positions || tall(Q, K));
+}
+bool sums_by_planes(size_t Q, size_t K, bool own_positions) { return own_positions ? K <= 63 && tall(Q, K) : K <= 127; }
 
 struct Plane {
   unsigned row[kEach], col[kEach];  // (of cells that are not there: the first)
@@ -603,8 +612,7 @@ Cut cut_for_bias(size_t B, size_t H, size_t Q, size_t K, size_t size) {
 Cut cut_for_planes(size_t B, size_t heads, size_t Q, size_t K, bool own_positions) {
   Cut c{};
   c.cols = (unsigned)K;
-  c.rows = kPlane / ((unsigned)K | 1);
-  if (c.rows > Q) c.rows = (unsigned)Q;
+  c.rows = (unsigned)plane_rows(Q, K);
   c.across = c.heads = c.parts = 1;
   c.strips = (unsigned)((Q + c.rows - 1) / c.rows);
   c.batches = own_positions ? 1 : (unsigned)B;
@@ -646,7 +654,7 @@ struct SumsCut {
   bool narrow;
   Cut cut;
   uint64_t groups;
-  SumsCut(size_t B, size_t H, size_t Q, size_t K, bool own_positions) : narrow(sums_by_planes(K, own_positions)) {
+  SumsCut(size_t B, size_t H, size_t Q, size_t K, bool own_positions) : narrow(sums_by_planes(Q, K, own_positions)) {
     if (narrow) {
       cut = cut_for_planes(B, H, Q, K, own_positions);
       groups = cut.tiles();
@@ -702,7 +710,7 @@ extern "C" int pskv_relbias(int device, void* stream, int type, const float* tab
     if (!same && a < o + out_bytes && o < a + extent(scores_stride, s, size))
       return set_error(PSKV_EINVAL, "out lies in the scores and is not the same tensor");
   }
-  const bool narrow = by_planes(Q, K, type_bytes(type), scores != nullptr);
+  const bool narrow = by_planes(Q, K, type_bytes(type), scores != nullptr, q_at != nullptr);
   Cut cut = narrow ? cut_for_planes(B, H, Q, K, q_at != nullptr) : cut_for_bias(B, H, Q, K, type_bytes(type));
   if (narrow) cut.heads = 1, cut.parts = (unsigned)H;
   if (cut.tiles() > kMostTiles) return set_error(PSKV_EINVAL, "sizes beyond what one call handles");

@@ -337,6 +337,9 @@ BIAS = [  # B, H, Q, K, buckets, far, two_sided, q_first, k_first, own positions
     (7, 3, 1, 100, 32, 128, False, 90, 0, False),
     (9, 2, 65, 63, 32, 128, True, 40, 0, True),
     (3, 2, 65, 64, 32, 128, True, 40, 0, True),
+    (9, 2, 64, 63, 32, 128, True, 40, 0, True),
+    (5, 2, 27, 20, 32, 128, True, 40, 0, True),
+    (5, 2, 28, 20, 32, 128, True, 40, 0, True),
     (5, 3, 26, 80, 32, 128, True, 0, 0, False),
     (5, 3, 26, 81, 32, 128, True, 0, 0, False),
     (5, 3, 21, 112, 32, 128, True, 0, 0, False),
