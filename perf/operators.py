@@ -190,15 +190,10 @@ def _prepare_dropout(case, g):
 
 # --- one pass ----------------------------------------------------------------------------------------------------
 
-_ops = None
-
-
 def run(state):
-    global _ops
     if own:
-        if _ops is None:  # (a program imports the package once, not with every call)
-            _ops = importlib.import_module("ps-lite_amd").ops
-        return globals()["_own_" + state["case"]["kind"]](state, _ops)
+        ops = importlib.import_module("ps-lite_amd").ops
+        return globals()["_own_" + state["case"]["kind"]](state, ops)
     return globals()["_plain_" + state["case"]["kind"]](state)
 
 
