@@ -756,6 +756,7 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
   bool narrow = false;
   Cut cut{};
   uint64_t groups = 0;
+  if (!any) work = nullptr;  // (nothing is summed up, and there are no strides)
   if (any) {
     if (!grad) return set_error(PSKV_EINVAL, "null buffer");
     if ((rc = check_strides("grad", grad_stride, s, false))) return rc;
