@@ -534,8 +534,9 @@ extern "C" int pskv_route_rows(int device, void* stream, int type, const void* x
   if (tokens == 0 || n_rows == 0) return PSKV_OK;
   if (!x || !place || !rows) return set_error(PSKV_EINVAL, "null buffer");
   const size_t size = type_bytes(type);
-  if (rows_overlap({x, tokens, k, x_stride, size}, {rows, n_rows, k, rows_stride, size}))
-    return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
+  const RowSpan to{rows, n_rows, k, rows_stride, size};
+  if (rows_overlap({x, tokens, k, x_stride, size}, to) || rows_overlap(stretch(place, tokens * choices * sizeof(int32_t)), to))
+    return set_error(PSKV_EINVAL, "the rows that are written overlap what is read");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   const RowArgs a = row_args(tokens, choices, n_rows, k, x_stride, rows_stride, type, lanes_of(tokens));

@@ -25,9 +25,12 @@ inline bool rows_overlap(const RowSpan& a, const RowSpan& b) {
   return in < a.k * a.size || in + b.k * b.size > s;
 }
 
+// A stretch of memory as one row (of nothing, if there is none).
+inline RowSpan stretch(const void* at, uint64_t bytes) { return {at, 1, at ? bytes : 0, 0, 1}; }
+
 // Whether two stretches of memory share a byte.
 inline bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
-  return rows_overlap({a, 1, a_bytes, 0, 1}, {b, 1, b_bytes, 0, 1});
+  return rows_overlap(stretch(a, a_bytes), stretch(b, b_bytes));
 }
 
 // How many lanes serve a row of `vectors` vectors: a power of two, at most `most`.

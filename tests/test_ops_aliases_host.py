@@ -1,11 +1,43 @@
 """What the operators on rows refuse of buffers that lie upon each other, without a GPU: no call here names a device that exists, so
 one that is not refused ends with PSKV_EHIP, and nothing is ever launched."""
+import ctypes
 import os
 import subprocess
 
 import pytest
 
 from conftest import REPO
+
+
+NOWHERE = -1  # a device that does not exist
+AT = [(i + 1) << 40 for i in range(8)]
+p = ctypes.c_void_p
+
+
+def refused(capi, code):
+    assert code in (capi.EINVAL, capi.EHIP)
+    return code == capi.EINVAL
+
+
+# --- tokens by expert --------------------------------------------------------------------------------------------
+
+T, CHOICES, K, ROWS = 10, 2, 16, 20  # float32: 10 rows of 64 bytes, 80 bytes of places or weights, 20 sorted rows
+
+
+def rows(capi, x=AT[0], place=AT[1], to=AT[2], to_stride=K):
+    return refused(capi, capi.load().pskv_route_rows(NOWHERE, None, 0, p(x), K, T, K, p(place), CHOICES, p(to), to_stride, ROWS))
+
+
+@pytest.mark.parametrize("offset", [-76, 0, 64, 20 * 64 - 4])
+def test_rows_refuse_their_places(capi, offset):
+    assert rows(capi, place=AT[2] + offset)
+
+
+@pytest.mark.parametrize("offset", [-80, 20 * 64])
+def test_rows_beside_their_places(capi, offset):
+    assert not rows(capi, place=AT[2] + offset)
+    # 80 bytes of places between rows 160 bytes apart
+    assert not rows(capi, place=AT[2] + 64, to_stride=40) and rows(capi, place=AT[2] + 60, to_stride=40) and rows(capi, place=AT[2] + 84, to_stride=40)
 
 
 # --- the gradient of the position bias ---------------------------------------------------------------------------
