@@ -563,8 +563,11 @@ extern "C" int pskv_route_sum(int device, void* stream, int type, const void* ro
   if (tokens == 0) return PSKV_OK;
   if ((n_rows && !rows) || !place || !out) return set_error(PSKV_EINVAL, "null buffer");
   const size_t size = type_bytes(type);
-  if (rows_overlap({rows, n_rows, k, rows_stride, size}, {out, tokens, k, out_stride, size}))
-    return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
+  const RowSpan to{out, tokens, k, out_stride, size};
+  const uint64_t listed = tokens * choices * 4;
+  if (rows_overlap({rows, n_rows, k, rows_stride, size}, to) || rows_overlap(stretch(place, listed), to) ||
+      rows_overlap(stretch(weights, listed), to))
+    return set_error(PSKV_EINVAL, "the rows that are written overlap what is read");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   // (without rows there is no row 0 to read either)

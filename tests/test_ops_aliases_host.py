@@ -40,6 +40,22 @@ def test_rows_beside_their_places(capi, offset):
     assert not rows(capi, place=AT[2] + 64, to_stride=40) and rows(capi, place=AT[2] + 60, to_stride=40) and rows(capi, place=AT[2] + 84, to_stride=40)
 
 
+def back(capi, answers=AT[0], place=AT[1], weights=AT[2], to=AT[3], to_stride=K):
+    return refused(capi, capi.load().pskv_route_sum(NOWHERE, None, 0, p(answers), K, ROWS, p(place), p(weights), CHOICES, p(to), to_stride, T, K))
+
+
+@pytest.mark.parametrize("what", ["place", "weights"])
+@pytest.mark.parametrize("offset", [-76, 0, 64, 10 * 64 - 4])
+def test_sum_refuses_its_places_and_weights(capi, what, offset):
+    assert back(capi, **{what: AT[3] + offset})
+
+
+@pytest.mark.parametrize("what", ["place", "weights"])
+def test_sum_beside_its_places_and_weights(capi, what):
+    assert not back(capi, **{what: AT[3] - 80}) and not back(capi, **{what: AT[3] + 640})
+    assert not back(capi, to_stride=40, **{what: AT[3] + 64}) and not back(capi, weights=None) and not back(capi, place=AT[2])
+
+
 # --- the gradient of the position bias ---------------------------------------------------------------------------
 
 @pytest.fixture(scope="module")
