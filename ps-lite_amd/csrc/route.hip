@@ -598,11 +598,13 @@ extern "C" int pskv_route_sum_grad(int device, void* stream, int type, const voi
   if (!grad || !place || !weights || !grad_weights || (n_rows && (!rows || !grad_rows)))
     return set_error(PSKV_EINVAL, "null buffer");
   const size_t size = type_bytes(type);
-  const RowSpan to{grad_rows, n_rows, k, grad_rows_stride, size};
-  if (overlap(weights, tokens * choices * 4, grad_weights, tokens * choices * 4))
-    return set_error(PSKV_EINVAL, "the weights and their gradients overlap");
-  if (rows_overlap({grad, tokens, k, grad_stride, size}, to) || rows_overlap({rows, n_rows, k, rows_stride, size}, to))
-    return set_error(PSKV_EINVAL, "the rows that are written overlap those that are read");
+  const uint64_t listed = tokens * choices * 4;
+  const RowSpan to{grad_rows, n_rows, k, grad_rows_stride, size}, to_weights = stretch(grad_weights, listed);
+  if (rows_overlap(to, to_weights)) return set_error(PSKV_EINVAL, "the gradients of the rows and of the weights overlap");
+  for (const RowSpan& read : {RowSpan{grad, tokens, k, grad_stride, size}, RowSpan{rows, n_rows, k, rows_stride, size},
+                              stretch(place, listed), stretch(weights, listed)})
+    if (rows_overlap(read, to) || rows_overlap(read, to_weights))
+      return set_error(PSKV_EINVAL, "the gradients that are written overlap what is read");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);
   RowArgs a = row_args(tokens, choices, n_rows, k, grad_stride, rows_stride, type, 64);

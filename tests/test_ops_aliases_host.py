@@ -56,6 +56,34 @@ def test_sum_beside_its_places_and_weights(capi, what):
     assert not back(capi, to_stride=40, **{what: AT[3] + 64}) and not back(capi, weights=None) and not back(capi, place=AT[2])
 
 
+GRAD = dict(grad=AT[0], answers=AT[1], place=AT[2], weights=AT[3], grad_rows=AT[4], grad_weights=AT[5], stride=K)
+
+
+def back_grad(capi, **change):
+    a = dict(GRAD, **change)
+    return refused(capi, capi.load().pskv_route_sum_grad(NOWHERE, None, 0, p(a["grad"]), K, T, K, p(a["answers"]), K, ROWS, p(a["place"]),
+                                                         p(a["weights"]), CHOICES, p(a["grad_rows"]), a["stride"], p(a["grad_weights"])))
+
+
+@pytest.mark.parametrize("what,size", [("place", 80), ("weights", 80), ("grad", 640), ("answers", 1280)])
+@pytest.mark.parametrize("written,room", [("grad_rows", 1280), ("grad_weights", 80)])
+def test_gradients_refuse_what_they_read(capi, what, size, written, room):
+    for offset in (4 - size, 0, 64, room - 4):
+        assert back_grad(capi, **{what: GRAD[written] + offset})
+    for offset in (-size, room):
+        assert not back_grad(capi, **{what: GRAD[written] + offset})
+
+
+def test_gradients_refuse_each_other(capi):
+    for offset in (-76, 0, 1276):
+        assert back_grad(capi, grad_weights=AT[4] + offset)
+    for offset in (-80, 1280):
+        assert not back_grad(capi, grad_weights=AT[4] + offset)
+    # between rows 160 bytes apart
+    for what in ("place", "weights", "grad_weights"):
+        assert not back_grad(capi, stride=40, **{what: AT[4] + 64}) and back_grad(capi, stride=40, **{what: AT[4] + 60})
+
+
 # --- the gradient of the position bias ---------------------------------------------------------------------------
 
 @pytest.fixture(scope="module")
