@@ -144,8 +144,11 @@ extern "C" int pskv_dropout(int device, void* stream, int type, const void* x, s
   if (!x || !out) return set_error(PSKV_EINVAL, "null buffer");
   const uint64_t blocks = (k + kDrawn - 1) / kDrawn;
   const bool in_place = x == out && (n == 1 || x_stride == out_stride);
-  if (!in_place && rows_overlap({x, n, k, x_stride, size}, {out, n, k, out_stride, size}))
+  const RowSpan to{out, n, k, out_stride, size};
+  if (!in_place && rows_overlap({x, n, k, x_stride, size}, to))
     return set_error(PSKV_EINVAL, "out overlaps x and is not the same rows");
+  if (rows_overlap(stretch(keys, n * sizeof(uint64_t)), to) || rows_overlap(stretch(step, sizeof(uint64_t)), to))
+    return set_error(PSKV_EINVAL, "out overlaps the keys or the step");
   const unsigned least = (unsigned)floor(p * 65536.0 + 0.5);
   const float scale = least < 65536 ? (float)(65536.0 / (65536 - least)) : 0.0f;
   DeviceGuard guard(device);

@@ -84,6 +84,24 @@ def test_gradients_refuse_each_other(capi):
         assert not back_grad(capi, stride=40, **{what: AT[4] + 64}) and back_grad(capi, stride=40, **{what: AT[4] + 60})
 
 
+# --- dropout -----------------------------------------------------------------------------------------------------
+
+def dropout(capi, x=AT[0], out=AT[1], keys=None, step=None, stride=16):
+    """10 rows of 16 float32."""
+    return refused(capi, capi.load().pskv_dropout(NOWHERE, None, 0, p(x), stride, p(out), stride, 10, 16, 0.5, 1, p(step), p(keys), 0))
+
+
+@pytest.mark.parametrize("what,size", [("keys", 80), ("step", 8)])
+def test_dropout_refuses_its_keys_and_step(capi, what, size):
+    for offset in (8 - size, 0, 64, 632):
+        assert dropout(capi, **{what: AT[1] + offset})
+        assert dropout(capi, x=AT[1], **{what: AT[1] + offset})  # in place, too
+    for offset in (-size, 640):
+        assert not dropout(capi, **{what: AT[1] + offset})
+    assert not dropout(capi, stride=40, **{what: AT[1] + 64})  # between rows 160 bytes apart
+    assert not dropout(capi, **{what: AT[0]})                  # both are read
+
+
 # --- the gradient of the position bias ---------------------------------------------------------------------------
 
 @pytest.fixture(scope="module")
