@@ -5,6 +5,7 @@
 // diagonals; the gradient's diagonals are summed into buckets once per tile.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <new>
 
 #include "host_common.h"
@@ -565,6 +566,14 @@ uint64_t extent(const int64_t* stride, const Shape& s, size_t size) {
   return ((s.B - 1) * (uint64_t)stride[0] + (s.H - 1) * (uint64_t)stride[1] + (s.Q - 1) * (uint64_t)stride[2] + s.K) * size;
 }
 
+// Whether a stretch of memory shares a byte with a [B, H, Q, K] tensor.
+bool lies_in(const void* at, uint64_t bytes, const void* tensor, const int64_t* stride, const Shape& s, size_t size) {
+  Nest dim[3] = {{s.B, (uint64_t)stride[0] * size}, {s.H, (uint64_t)stride[1] * size}, {s.Q, (uint64_t)stride[2] * size}};
+  std::sort(dim, dim + 3, [](const Nest& a, const Nest& b) { return a.stride > b.stride; });
+  const uint64_t first = reinterpret_cast<uintptr_t>(at);
+  return touches(first, first + bytes, reinterpret_cast<uintptr_t>(tensor), dim, 3, s.K * size);
+}
+
 int check_strides(const char* what, const int64_t* stride, const Shape& s, bool written) {
   if (!stride) return set_error(PSKV_EINVAL, "%s: no strides", what);
   uint64_t n[4] = {s.B, s.H, s.Q, s.K}, by[4] = {(uint64_t)stride[0], (uint64_t)stride[1], (uint64_t)stride[2], 1};
@@ -772,8 +781,13 @@ extern "C" int pskv_relbias_grad(int device, void* stream, int type, const void*
     else if (!work || work_bytes < room || (reinterpret_cast<uintptr_t>(work) & 3))
       return set_error(PSKV_EINVAL, "this gradient takes %zu bytes of working memory, %zu given", room, work ? work_bytes : (size_t)0);
   }
-  if (work && (overlap(work, groups * buckets * H * sizeof(float), grad_table, buckets * H * sizeof(float)) ||
-              overlap(work, groups * buckets * H * sizeof(float), grad, extent(grad_stride, s, type_bytes(type)))))
+  const uint64_t table_bytes = buckets * H * sizeof(float), used = work ? groups * table_bytes : 0;
+  if (any && lies_in(grad_table, table_bytes, grad, grad_stride, s, type_bytes(type)))
+    return set_error(PSKV_EINVAL, "the gradient of the table lies in the gradient that is read");
+  if (any && q_at && (overlap(q_at, B * sizeof(int64_t), grad_table, table_bytes) || overlap(q_at, B * sizeof(int64_t), work, used)))
+    return set_error(PSKV_EINVAL, "the gradient of the table or the working memory overlaps the positions");
+  if (work && (overlap(work, used, grad_table, table_bytes) ||
+              overlap(work, used, grad, extent(grad_stride, s, type_bytes(type)))))
     return set_error(PSKV_EINVAL, "the working memory overlaps the gradients");
   DeviceGuard guard(device);
   if (!guard.ok()) return set_error(PSKV_EHIP, "cannot select device %d", device);

@@ -4,6 +4,7 @@ import ctypes
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 from conftest import REPO
@@ -121,3 +122,59 @@ def test_empty_gradient_with_working_memory(capi, entry, shape):
     """A gradient of nothing has no strides to be looked at."""
     done = subprocess.run([entry] + [str(x) for x in shape], capture_output=True, text=True)
     assert done.returncode == 0 and done.stdout.split() == [str(capi.EHIP)], done
+
+
+def strides(*by):
+    return (ctypes.c_int64 * 3)(*by)
+
+
+BIAS_GRAD = dict(grad=AT[0], by=(400, 100, 10), at=None, B=2, Q=10, K=10, table=AT[1], work=AT[2], size=4)
+
+
+def bias_grad(capi, **change):
+    """4 heads, 32 buckets: a gradient of 512 bytes."""
+    a = dict(BIAS_GRAD, **change)
+    types = {4: 0, 2: 1}
+    return refused(capi, capi.load().pskv_relbias_grad(NOWHERE, None, types[a["size"]], p(a["grad"]), strides(*a["by"]), 32, 4, 128, 1, 0, 0, p(a["at"]),
+                                                       a["B"], a["Q"], a["K"], p(a["table"]), p(a["work"]), 1 << 20))
+
+
+def test_bias_gradient_refuses_what_it_reads(capi):
+    size = 2 * 400 * 4
+    for offset in (-508, 0, 1600, size - 4):
+        assert bias_grad(capi, table=AT[0] + offset)
+    for offset in (-512, size):
+        assert not bias_grad(capi, table=AT[0] + offset)
+    for offset in (-8, 0, 504):  # 16 bytes of positions
+        assert bias_grad(capi, at=AT[1] + offset)
+    for offset in (-16, 512):
+        assert not bias_grad(capi, at=AT[1] + offset)
+
+
+def test_bias_gradient_and_its_working_memory(capi):
+    lib = capi.load()
+    many = dict(B=40)  # takes working memory, with positions and without
+    room = lib.pskv_relbias_grad_room(32, 4, 40, 10, 10, 1)
+    assert room >= 512
+    for offset in (-312, 0, room - 8):  # 320 bytes of positions
+        assert bias_grad(capi, at=AT[2] + offset, **many)
+    for offset in (-320, room):
+        assert not bias_grad(capi, at=AT[2] + offset, **many)
+
+
+def test_bias_gradient_beside_what_it_reads(capi):
+    """512 bytes between the sequences, heads or queries of a gradient, whose dimensions lie in any order."""
+    rng = np.random.default_rng(5)
+    for _ in range(3000):
+        B, Q, K, size = int(rng.integers(1, 4)), int(rng.integers(1, 4)), int(rng.integers(1, 40)), int(rng.choice([2, 4]))
+        n, by, reach = {0: B, 1: 4, 2: Q}, [0, 0, 0], K
+        for d in rng.permutation(3):
+            by[d] = int(reach + rng.choice([0, 3, 700]))
+            reach = (n[d] - 1) * by[d] + reach
+        if rng.random() < 0.2:
+            by[int(rng.integers(0, 3))] = 0  # (of a gradient that is expanded)
+        starts = np.add.outer(np.add.outer(np.arange(B) * by[0], np.arange(4) * by[1]), np.arange(Q) * by[2]).ravel() * size
+        offset = 4 * int(rng.integers(-140, reach * size // 4 + 10))
+        share = bool(np.any((starts < offset + 512) & (starts + K * size > offset)))
+        got = bias_grad(capi, B=B, Q=Q, K=K, size=size, by=by, table=AT[0] + offset)
+        assert got == share, (B, Q, K, size, by, offset)
