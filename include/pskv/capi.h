@@ -346,7 +346,7 @@ int pskv_route_sum_grad(int device, void* stream, int type, const void* grad, si
  * one-sided: key positions behind the query's share bucket 0. Of the m buckets of a side the first m / 2 are for one distance
  * each; the others widen in a geometric progression up to max_distance and the last one takes what lies beyond. Borders are
  * found in whole numbers: bucket m / 2 + c begins at the least d with d^(m - m/2) >= (m/2)^(m - m/2 - c) max_distance^c.
- * q_at (device, B entries) may be NULL: 0. scores may be NULL: the bias alone; scores may be out itself. Strides are host
+ * q_at (device, B entries of any value) may be NULL: 0. scores may be NULL: the bias alone; scores may be out itself. Strides are host
  * arrays of three (batch, head, row; the scores' may be 0, for what a batch or all heads share). Sums in float, one rounding. */
 #define PSKV_RELBIAS_MAX_BUCKETS 256
 int pskv_relbias(int device, void* stream, int type, const float* table, size_t buckets, size_t H, uint64_t max_distance,

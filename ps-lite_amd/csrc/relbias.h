@@ -39,6 +39,14 @@ PSKV_BOTH inline int32_t nearer(int64_t rel) {
   return rel > most ? (int32_t)most : rel < -most ? (int32_t)-most : (int32_t)rel;
 }
 
+// The same of rel0 - own + step: rel0 up to 2^61 and step up to 2^32 either way, `own` (a sequence's position) any number. From 2^62 on it
+// alone decides on which side and that it is far.
+PSKV_BOTH inline int32_t nearer(int64_t rel0, int64_t own, int64_t step) {
+  const int64_t most = 1ll << 62;
+  own = own > most ? most : own < -most ? -most : own;
+  return nearer(rel0 - own + step);
+}
+
 // The row of a relative position. The logarithm in float tells where to look: its error, some 1e-6, times at most 11,400 buckets per
 // doubling is far below one, so the bucket is the one that it says or a neighbour, and the borders decide. `border` is b.border
 // with 0 in front and the largest number behind, where it can be read fastest.

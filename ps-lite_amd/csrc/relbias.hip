@@ -190,7 +190,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias(const float* __restrict__ ta
   for (unsigned tile = blockIdx.x * kWaves + wave; tile < tiles; tile += gridDim.x * kWaves) {
     const Tile t(tile, cut, s);
     const Span<N> span(t.c0, lane, s.K);
-    const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0));
+    const int32_t rel = nearer(s.rel0, q_at ? q_at[t.batch0] : 0, (int64_t)(t.c0 - t.r0));
     unsigned row[N];  // of the table
 #pragma unroll
     for (unsigned k = 0; k < N; ++k) row[k] = bucket_of(b, border, rel + (int)(lane * N + k)) * (unsigned)s.H;
@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias_step(const float* __restrict
       Some<T, N> x[kGroup];
       if (SCORES)
         span.template load<WHOLE, false>(x, scores + t.batch0 * s.in[0] + t.head0 * s.in[1], s.in[1], t.heads);
-      const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0));
+      const int32_t rel = nearer(s.rel0, q_at ? q_at[t.batch0] : 0, (int64_t)t.c0);
       unsigned row[N];
 #pragma unroll
       for (unsigned k = 0; k < N; ++k) row[k] = bucket_of(b, border, rel + (int)(lane * N + k)) * (unsigned)s.H + t.head0;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias_narrow(const float* __restri
   for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const Tile t(tile, cut, s);
     const Plane c(t.rows, K);
-    const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) - t.r0 - (t.rows - 1)));
+    const int32_t rel = nearer(s.rel0, q_at ? q_at[t.batch0] : 0, (int64_t)(0 - t.r0 - (t.rows - 1)));
     __syncthreads();
     for (unsigned x = threadIdx.x; x < t.rows + K - 1; x += kBlock)
       bias[x] = table[bucket_of(b, border, rel + (int)x) * (unsigned)s.H + t.head0];
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias_sums(const T* __restrict__ g
     for (unsigned k = 0; k < kWide; ++k) diagonal[wave][lane * kWide + k] = high[k];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // diagonal[x] is the one that is x - reach columns to the right of the tile's corner
-    const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) + t.c0 - t.r0 - reach));
+    const int32_t rel = nearer(s.rel0, q_at ? q_at[t.batch0] : 0, (int64_t)(t.c0 - t.r0 - reach));
     // (those that no element of the tile is on are left out)
     const unsigned reached = reach + (s.K - t.c0 < kCols ? (unsigned)(s.K - t.c0) : kCols);
     add_buckets(sums[wave], b, border, rel, 0, 64, reached, [&](unsigned x) { return diagonal[wave][x]; });
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(kBlock) void k_relbias_narrow_sums(const T* __restr
     if (c.has(i)) plane[c.row[i] * pitch + c.col[i]] = sum[i];
   __syncthreads();
   // diagonal x begins at column x - (rows - 1) of row 0, or at column 0 of row rows - 1 - x
-  const int32_t rel = nearer((int64_t)((uint64_t)s.rel0 - (q_at ? (uint64_t)q_at[t.batch0] : 0) - t.r0 - (t.rows - 1)));
+  const int32_t rel = nearer(s.rel0, q_at ? q_at[t.batch0] : 0, (int64_t)(0 - t.r0 - (t.rows - 1)));
   add_buckets(sums[wave], b, border, rel, wave * 64, kBlock, t.rows + K - 1, [&](unsigned x) {
     const unsigned r = x < t.rows ? t.rows - 1 - x : 0, k = x < t.rows ? 0 : x - (t.rows - 1);
     const unsigned cells = t.rows - r < K - k ? t.rows - r : K - k;
