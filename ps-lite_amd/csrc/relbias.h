@@ -40,11 +40,12 @@ PSKV_BOTH inline int32_t nearer(int64_t rel) {
 }
 
 // The same of rel0 - own + step: rel0 up to 2^61 and step up to 2^32 either way, `own` (a sequence's position) any number. From 2^62 on it
-// alone decides on which side and that it is far.
+// alone decides on which side and that it is far, so its upper word may be brought nearer (two instructions of the scalar unit, which does not
+// compare 64 bits).
 PSKV_BOTH inline int32_t nearer(int64_t rel0, int64_t own, int64_t step) {
-  const int64_t most = 1ll << 62;
-  own = own > most ? most : own < -most ? -most : own;
-  return nearer(rel0 - own + step);
+  const int32_t most = 1 << 30, upper = (int32_t)(own >> 32);
+  const int32_t near = upper > most ? most : upper < -most ? -most : upper;
+  return nearer(rel0 - (int64_t)((uint64_t)(uint32_t)near << 32 | (uint32_t)own) + step);
 }
 
 // The row of a relative position. The logarithm in float tells where to look: its error, some 1e-6, times at most 11,400 buckets per
