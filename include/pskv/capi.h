@@ -304,7 +304,9 @@ int pskv_match(int device, const uint64_t* src_keys, size_t n_src, const float* 
  *    capture). Calls share no state: several may run at once, from several threads, and two recorded graphs need only
  *    working memory (`work`) of their own. Buffers stay the caller's to keep until the stream has run the call.
  *  - What the host can see is checked before anything is enqueued (PSKV_EINVAL); indexes that lie in device memory are checked
- *    by the kernels, so no value of theirs leads outside the buffers that the call was given.
+ *    by the kernels, so no value of theirs leads outside the buffers that the call was given. What a call writes may share no byte
+ *    with what it reads or with anything else that it writes, but where an answer is said to go to its own input; rows between
+ *    each other's (columns of one matrix) share none.
  *  - `type` is the type of the rows' elements. Sums are taken in float in a fixed order and rounded once (to nearest, ties to
  *    even): the same inputs give the same bits. Strides count elements; the elements of a row lie side by side; rows may begin
  *    anywhere that an element may. */
@@ -324,7 +326,9 @@ int pskv_route_sort(int device, void* stream, const void* experts, int index_bit
                     int32_t* place, int32_t* offsets, void* work, size_t work_bytes);
 
 /* Every token's row goes to its places: rows[place[t*choices + j]] = x[t]. Places outside [0, n_rows) are skipped, rows that no
- * place names are left as they are. The gradient of x is pskv_route_sum of the rows' gradient, without weights. */
+ * place names are left as they are (those behind the last expert's hold what an earlier call wrote there). Places name a row once at
+ * most, as those of pskv_route_sort do; of several rows that go to one place, which remains is not determined. The gradient of x is
+ * pskv_route_sum of the rows' gradient, without weights. */
 int pskv_route_rows(int device, void* stream, int type, const void* x, size_t x_stride, size_t tokens, size_t k,
                     const int32_t* place, size_t choices, void* rows, size_t rows_stride, size_t n_rows);
 
@@ -335,7 +339,8 @@ int pskv_route_sum(int device, void* stream, int type, const void* rows, size_t 
                    size_t k);
 
 /* The gradient of pskv_route_sum: grad_rows[place] = weight * grad[t] (rows that no place names are left as they are) and
- * grad_weights[t*choices + j] = <grad[t], rows[place]>, 0 for a place outside [0, n_rows). */
+ * grad_weights[t*choices + j] = <grad[t], rows[place]>, 0 for a place outside [0, n_rows). A row that several choices name gets the
+ * gradient of one of them, not their sum: places name a row once at most, as those of pskv_route_sort do. */
 int pskv_route_sum_grad(int device, void* stream, int type, const void* grad, size_t grad_stride, size_t tokens, size_t k,
                         const void* rows, size_t rows_stride, size_t n_rows, const int32_t* place, const float* weights,
                         size_t choices, void* grad_rows, size_t grad_rows_stride, float* grad_weights);
@@ -364,10 +369,12 @@ int pskv_relbias_grad(int device, void* stream, int type, const void* grad, cons
 
 /* Dropout of n rows of k elements: out = x * scale where the element is kept, 0 where it is dropped (whatever x is there). Nothing
  * is stored: whether column c of a row is kept is drawn from the row's 64-bit key (keys[r], or first + r with keys == NULL),
- * c and the seed, so the gradient is the same call on the gradient's rows, in any order, in any pieces. 16 bits b of
+ * c and the seed, so the gradient is the same call on the gradient's rows, in any order, in any pieces of whole rows. 16 bits b of
  * Philox4x32-10 (key: seed low, high; counter: row key low, high, c / 8, 0; the 8 columns take the halves of its four words,
  * low ones first) are compared with least = p * 65536 rounded to the nearest: kept where b >= least, scale = 65536 / (65536 -
  * least). step (device, one word, may be NULL) is added to the seed: a recorded graph draws anew where the program changes it.
+ * Their sum is what counts: two seeds d apart draw the same masks d steps apart, so calls that share a step and have keys in common
+ * take seeds that lie further apart than there are steps (64 random bits each do, numbers of layers do not).
  * out may be x itself. */
 int pskv_dropout(int device, void* stream, int type, const void* x, size_t x_stride, void* out, size_t out_stride, size_t n,
                  size_t k, double p, uint64_t seed, const uint64_t* step, const uint64_t* keys, uint64_t first);

@@ -5,7 +5,8 @@ include/pskv/capi.h).
 Arguments are torch tensors on one GPU; a call fills the tensors that it is given for its answers. Rows are float32, float16
 or bfloat16, the elements of a row lie side by side, rows may be any number of elements apart. A call is enqueued on torch's
 current stream of that GPU, or on `stream` (the address of a hipStream_t), waits for nothing and may be captured into a
-graph (after a first call outside any capture). With a `stream` of one's own, tensors have to be complete on it and to be
+graph (after a first call outside any capture). What a call writes may share no memory with what it reads, but where an answer may be
+its own input. With a `stream` of one's own, tensors have to be complete on it and to be
 kept until it has run the call.
 
 These are calls, not nodes of autograd: a gradient is the call that is named as such. Tensors that do not fit raise TypeError
@@ -50,8 +51,9 @@ def route_sort(experts, num_experts, order, place, offsets, work=None, stream=No
 
 
 def route_rows(x, place, rows, stream=None):
-    """rows[place[t, j]] = x[t]: every token's row ([tokens, k]) goes to the places of its choices. Rows that no place names
-    are left as they are. The gradient of x is route_sum(grad of rows, place, grad of x)."""
+    """rows[place[t, j]] = x[t]: every token's row ([tokens, k]) goes to the places of its choices, which name a row once at most.
+    Rows that no place names are left as they are: those behind the last expert's hold what an earlier call wrote there. The gradient
+    of x is route_sum(grad of rows, place, grad of x)."""
     rc = _native().route_rows(x, place, rows, stream)
     if rc:
         _check(rc)
@@ -67,7 +69,8 @@ def route_sum(rows, place, out, weights=None, stream=None):
 
 def route_sum_grad(grad, rows, place, weights, grad_rows, grad_weights, stream=None):
     """The gradient of route_sum: grad_rows[place[t, j]] = weights[t, j] * grad[t] and grad_weights[t, j] = <grad[t],
-    rows[place[t, j]]> (float32, 0 for a choice that is not here). Rows that no place names are left as they are."""
+    rows[place[t, j]]> (float32, 0 for a choice that is not here). Rows that no place names are left as they are. A row that
+    several choices name gets the gradient of one of them: places are those of route_sort, which name a row once at most."""
     rc = _native().route_sum_grad(grad, rows, place, weights, grad_rows, grad_weights, stream)
     if rc:
         _check(rc)
@@ -109,7 +112,8 @@ def dropout(x, out, p, seed, keys=None, first=0, step=None, stream=None):
     """out = x * scale where an element is kept, 0 where it is dropped, with probability p (to 16 bits). Whether an element is
     kept depends on seed (0 .. 2^64 - 1), on its row's key (keys: int64, [rows]; else first, first + 1, ...) and its column
     alone, so the gradient is the same call on the gradient's rows, in any order. step (one int64 on the GPU) is added to the
-    seed, for graphs that draw anew at every replay. out may be x."""
+    seed, for graphs that draw anew at every replay: seeds that share a step lie further apart than there are steps (random ones do),
+    or one draws what the other drew some steps before. out may be x."""
     rc = _native().dropout(x, out, p, seed, step, keys, first, stream)
     if rc:
         _check(rc)
