@@ -39,7 +39,7 @@ struct Divisor {
 };
 
 // 16-bit types: a lane takes the 8 columns of a draw, 16 bytes. Indexes are those of draws. The ten rounds' products (16 cycles each)
-// and the memory take about the same time: 65,536 rows of 2,048 bf16 in 90 us, 6.0 TB/s; 4,099 of 1,001 in 5.5.
+// and the memory take about the same time: 65,536 rows of 2,048 bf16 in 90 us, 6.0 TB/s; 4,099 of 1,001 in 5.9 to 6.4 us.
 template <typename T, bool PAST>
 __global__ __launch_bounds__(kBlock) void k_dropout(const T* x, T* out, const uint64_t* __restrict__ keys, uint64_t first,
                                                      const uint64_t* __restrict__ step, uint64_t seed, uint32_t draws, uint32_t k,

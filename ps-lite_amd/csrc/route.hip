@@ -5,7 +5,8 @@
 //     rows[place]   = x[t]                              its gradient: dx[t] = sum_j drows[place[t,j]]
 //     y[t]          = sum_j w[t,j] answers[place[t,j]]  its gradient: danswers[place] = w dy[t], dw[t,j] = <dy[t], answers[place]>
 // Everything but the sort goes token by token: a token's own row is read or written once, its K others once each, nothing is
-// summed by more than one wavefront, and no sum depends on the order in which workgroups run.
+// summed by more than one wavefront, and no sum depends on the order in which workgroups run. (The gradient of y reads a token's row once
+// for every wavefront that its choices are shared out to, and once for every choice where it is longer than 256 vectors of 16 bytes.)
 #include <hip/hip_runtime.h>
 
 #include "host_common.h"
@@ -85,8 +86,8 @@ __global__ __launch_bounds__(kSortBlock) void k_route_scan(unsigned* __restrict_
 
 // Places of a tile's choices. A wavefront owns neighbouring ones and takes them 64 at a time: lanes of the same bin find each
 // other by comparing the bits of their bins, so a choice's rank among its wavefront's is known without atomics; ranks begin
-// where the earlier wavefronts', tiles' and bins' choices end. 16 choices take 2.8 us, 15,009 of 64 experts 6.8 with their counts,
-// 262,144 of 256 13.3: a chain of steps that each wait for the one before, on as many compute units as there are tiles (every workgroup
+// where the earlier wavefronts', tiles' and bins' choices end. 16 choices take 2.9 us; with their counts, in a graph of sorts, 15,009 of
+// 64 experts 7.0 and 262,144 of 256 13.3 (in a trace the kernels' own times add up to 7.7 to 8.3 and 16.0): a chain of steps that each wait for the one before, on as many compute units as there are tiles (every workgroup
 // counting all choices itself instead of a launch for the counts: twice the time where half of them are of one expert, for the atomics
 // on one counter).
 template <typename I, unsigned ITEMS>
@@ -205,8 +206,11 @@ __global__ __launch_bounds__(kSortBlock) void k_route_place(const I* __restrict_
 
 // --- rows out and back -------------------------------------------------------------------------------------------
 
-// All three kernels move what they have to and nothing else (read and written at the memory: 1.00 of it), so the memory bounds them where
-// there are many tokens: 32,768 x 8 rows of 2,048 bf16 out at 5.3 TB/s (1.2 GB in 229 us; rows of 4 KB that go to eight places) and
+// Where there are many tokens and rows are whole lines, all three kernels move what they have to and nothing else (read and written at the
+// memory: 1.00 of it, the gradient up to 256 vectors a row), so the memory bounds them. Rows that begin and end inside lines move some
+// 10 % more (3 x 5,003 rows of 1,001 float16: 10.8 MB read for 10.0 out, 26.4 for 24.0 back; the gradient of 6 x 1,999 of 777 float32, whose token's
+// row is read by every wavefront that has some of its choices: 45.5 for 39.9), and their last elements, fewer than a vector, are asked for
+// choice by choice, each behind the one before. 32,768 x 8 rows of 2,048 bf16 out at 5.3 TB/s (1.2 GB in 229 us; rows of 4 KB that go to eight places) and
 // back at 5.8 (210 us), the gradient of 16,384 x 4 at 5.5 (111 us). Calls that move more than the memory-side cache holds go
 // past it (back: 280 -> 211 us; the gradient and the sum of its rows 178 -> 165); smaller ones leave it their rows, which the
 // next call wants (36 MB past it: 8.4 -> 10.8 us out, 8.9 -> 9.7 back).
@@ -317,7 +321,9 @@ __global__ __launch_bounds__(kRowBlock) void k_route_sum(const T* __restrict__ r
 
 // At most a wavefront per token, so that the products' sums need no other than its own lanes. A lane keeps its part of the
 // token's gradient, NV vectors of it, for all its choices (`share` of them, all where there are many tokens), and asks for four
-// vectors of the answers at once, of 4 / NV choices. Rows of more than 4 x 64 vectors (LONG) go piece by piece.
+// vectors of the answers at once, of 4 / NV choices. Rows of more than 4 x 64 vectors (LONG) go piece by piece, and the token's
+// gradient is asked for anew with every choice: 8,192 x 4 of 4,096 bf16 128 us, of 2,048 float32 123, 487 MB read for 336 (some of it again from
+// the caches), where 16,384 x 4 of 2,048 bf16, as many bytes, take 111.
 constexpr unsigned kKept = 4;
 
 template <typename T, bool ONE, bool PAST, unsigned NV, bool LONG>
@@ -430,7 +436,7 @@ int check_stride(const char* what, uint64_t n, uint64_t k, uint64_t stride, bool
 }
 
 // How a sort is cut into tiles: 1, 2 or 4 choices to each of a workgroup's 1,024 lanes. One tile, and one launch, up to 4,096. From
-// there on as small tiles as there may be, for a tile's steps are what takes the time (15,009 choices of 64 experts: 6.8 us
+// there on as small tiles as there may be, for a tile's steps are what takes the time (in a graph of sorts, 15,009 choices of 64 experts: 6.8 us
 // with one choice to a lane, 7.5 with two, 9.5 with four; 262,144 of 256: 13.3 with two, 13.7 with four), until adding up the tiles' counts
 // takes longer (524,288 of 256: 21.2, 15.4, 16.9; 1,048,576 of 64: two 22.9, four 16.3).
 struct SortCut {
